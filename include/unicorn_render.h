@@ -290,6 +290,37 @@ int ur_render_meshes_backward(const float* grad_image, const float* verts, const
                               float* grad_face_verts, float* grad_maps, int grads_are_zero, float* grad_verts,
                               float* grad_R, float* grad_T, void* stream);
 
+/* ======================================================================================================================
+ * Operators of the networks around the renderer: what predicts the poses it renders and learns from the result.
+ * No counterpart in the reference's native layer (its heads are torch modules; it renders EVERY candidate pose,
+ * unicorn.py:295-304, utils/mesh.py:43-71).  Conventions as above, except that tensors may be fp32, fp16 or bf16
+ * (UR_F32 / UR_F16 / UR_BF16); sums and statistics are fp32 or wider, a result is rounded to its type once.  Rows may
+ * start anywhere (any stride, any alignment of their element type).  Nothing is summed by floating-point atomics: the
+ * same call gives the same bits.
+ * ==================================================================================================================== */
+#define UR_F32 0
+#define UR_F16 1
+#define UR_BF16 2
+
+/*
+ * Layer normalisation over the last dimension: y = (x - mean) / sqrt(var + eps) * weight + bias, row by row.
+ *   x: `rows` rows of `cols` elements, row i at x + i * x_row_stride (elements; at least cols) ; weight, bias (cols) of type
+ *   param_dtype (dtype or UR_F32), either may be NULL ; y (rows, cols) contiguous, of type dtype ;
+ *   mean, rstd (rows) fp32: kept for the backward, NULL together when there will be none.
+ * Backward: grad_y as x (own stride) -> grad_x (rows, cols), grad_weight, grad_bias (cols, param_dtype: sums over the
+ *   rows in a fixed order); each may be NULL.
+ * workspace: ur_layer_norm_workspace_bytes(rows, cols, dtype, backward) of uninitialised memory (0 is possible in the
+ *   forward: then NULL will do); negative = error.
+ */
+int64_t ur_layer_norm_workspace_bytes(int64_t rows, int64_t cols, int dtype, int backward);
+int ur_layer_norm_forward(const void* x, int64_t x_row_stride, const void* weight, const void* bias, int dtype,
+                          int param_dtype, int64_t rows, int64_t cols, float eps, void* y, float* mean, float* rstd,
+                          void* workspace, size_t workspace_bytes, void* stream);
+int ur_layer_norm_backward(const void* grad_y, int64_t grad_row_stride, const void* x, int64_t x_row_stride,
+                           const void* weight, const float* mean, const float* rstd, int dtype, int param_dtype,
+                           int64_t rows, int64_t cols, void* grad_x, void* grad_weight, void* grad_bias,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,80 @@
+"""What the operators of the networks around the renderer refuse, checked without a GPU: their Python checks run before
+anything touches a device, and the C entry points answer bad arguments with a code and a message before any launch (the
+pointers below are never read)."""
+import pytest
+import torch
+
+from unicorn_amd import native
+
+FAKE = 4096  # a pointer that is not null; no call below gets as far as a launch
+
+
+def refused(name, *args):
+    rc = getattr(native.lib(), name)(*args)
+    message = native.lib().ur_last_error().decode()
+    assert rc < 0 and message, name
+    return rc, message
+
+
+def test_layer_norm_python_checks():
+    from unicorn_amd.normalization import LayerNorm, layer_norm
+    x = torch.randn(4, 8)
+    with pytest.raises(ValueError, match="GPU"):
+        layer_norm(x)
+    with pytest.raises(ValueError, match="GPU"):
+        layer_norm(x.requires_grad_(True))
+    for bad in (torch.randn(4, 8).double(), torch.ones(4, 8, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
+            layer_norm(bad)
+    with pytest.raises(ValueError, match="at least 1"):
+        layer_norm(torch.empty(4, 0))
+    with pytest.raises(ValueError, match="at least 1"):
+        layer_norm(torch.tensor(1.0))
+    with pytest.raises(ValueError, match="weight must have shape"):
+        layer_norm(x, torch.ones(7))
+    with pytest.raises(ValueError, match="bias must have shape"):
+        layer_norm(x, None, torch.ones(1, 8))
+    with pytest.raises(ValueError, match="weight must be"):
+        layer_norm(x, torch.ones(8).half())
+    with pytest.raises(ValueError, match="same type"):
+        layer_norm(x.half(), torch.ones(8).half(), torch.ones(8))
+    for eps in (-1e-5, float("nan")):
+        with pytest.raises(ValueError, match="eps"):
+            layer_norm(x, eps=eps)
+    with pytest.raises(ValueError, match="dim"):
+        LayerNorm(0)
+
+
+def test_layer_norm_entry_point_checks():
+    fwd = lambda x=FAKE, stride=8, w=None, b=None, dt=0, pdt=0, M=4, D=8, eps=1e-5, y=FAKE, mean=None, rstd=None, ws=None, n=0: (  # noqa: E731
+        "ur_layer_norm_forward", x, stride, w, b, dt, pdt, M, D, eps, y, mean, rstd, ws, n, None)
+    assert refused(*fwd(x=None))[0] == -1
+    assert refused(*fwd(y=None))[0] == -1
+    assert "dtype" in refused(*fwd(dt=3))[1]
+    assert "type" in refused(*fwd(dt=1, pdt=2))[1]
+    assert refused(*fwd(M=0))[0] == -1 and refused(*fwd(D=0))[0] == -1 and refused(*fwd(M=-1))[0] == -1
+    assert refused(*fwd(M=1 << 31))[0] == -2 and refused(*fwd(D=1 << 31, stride=1 << 31))[0] == -2
+    assert "stride" in refused(*fwd(stride=7))[1]
+    assert "eps" in refused(*fwd(eps=-1.0))[1] and "eps" in refused(*fwd(eps=float("nan")))[1]
+    assert "together" in refused(*fwd(mean=FAKE))[1]
+    assert refused(*fwd(D=1 << 20, stride=1 << 20))[0] == -4          # long rows need a workspace
+    n = native.lib().ur_layer_norm_workspace_bytes(4, 8, 0, 1)
+    bwd = lambda dy=FAKE, gs=8, x=FAKE, mean=FAKE, rstd=FAKE, gx=FAKE, gw=FAKE, gb=FAKE, ws=FAKE, n=n: (  # noqa: E731
+        "ur_layer_norm_backward", dy, gs, x, 8, None, mean, rstd, 0, 0, 4, 8, gx, gw, gb, ws, n, None)
+    for k in ("dy", "x", "mean", "rstd"):
+        assert refused(*bwd(**{k: None}))[0] == -1
+    assert "no gradient" in refused(*bwd(gx=None, gw=None, gb=None))[1]
+    assert "stride" in refused(*bwd(gs=7))[1]
+    assert refused(*bwd(n=n - 1))[0] == -4 and refused(*bwd(ws=None))[0] == -4
+    for args in ((0, 8, 0, 0), (4, 0, 0, 0), (4, 8, 3, 0), (1 << 31, 8, 0, 1)):
+        assert refused("ur_layer_norm_workspace_bytes", *args)[0] == -1
+
+
+def test_layer_norm_workspace_sizes():
+    size = native.lib().ur_layer_norm_workspace_bytes
+    for dt in (0, 1, 2):
+        assert size(5, 64, dt, 0) == 0                                 # rows that fit registers: nothing kept
+        for M, D in ((1, 1), (7, 33), (100000, 64), (3, 1 << 20), (1, (1 << 31) - 1)):
+            n = size(M, D, dt, 1)
+            assert n >= 2 * D * 4 and n % 4 == 0                        # at least one row of partial sums
+            assert size(M, D, dt, 0) <= n

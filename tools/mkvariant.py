@@ -3,12 +3,11 @@
 usage: mkvariant.py name 'old1=>new1' 'old2=>new2' ...   (each `old` must occur exactly once; @@ stands for a newline)
 Output: abx/<name>.hip, abx/lib<name>.so.  Timing experiments only -- a variant may compute wrong numbers."""
 import os
-import subprocess
 import sys
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, ROOT)
-from __graft_entry__ import HIPCC, HIP_FLAGS, SRC  # noqa: E402
+from __graft_entry__ import SRC, compile_library  # noqa: E402
 
 
 def main():
@@ -26,7 +25,7 @@ def main():
     src = src.replace('#include "../../include/unicorn_render.h"', f'#include "{ROOT}/include/unicorn_render.h"')
     src = src.replace('#include "ur_device.h"', f'#include "{ROOT}/unicorn_amd/csrc/ur_device.h"')
     open(path, "w").write(src)
-    subprocess.check_call([HIPCC] + HIP_FLAGS + ["-o", os.path.join(ROOT, "abx", f"lib{name}.so"), path])
+    compile_library(os.path.join(ROOT, "abx", f"lib{name}.so"), render_src=path)
     print("built", name)
 
 

@@ -1,0 +1,563 @@
+// ur_layer_norm.hip -- layer normalisation over the last dimension, forward and backward, with the sums of the
+// weight's and the bias's gradients.
+//
+//   m = sum(x) / D      v = sum((x - m)^2) / D      r = 1 / sqrt(v + eps)      h = (x - m) r      y = h w + b
+//   g = dy w            dx = r (g - mean(g) - h mean(g h))          dw = sum_rows(dy h)       db = sum_rows(dy)
+//
+// Everything is bound by memory: x is read once (dy too in the backward) and one result written, so a row stays in
+// registers between its statistics and its result.  Statistics, sums and the arithmetic are fp32; a result is rounded to
+// its type once.  The variance is the sum of squared differences from the mean already known (two passes over
+// registers), not E[x^2] - m^2, which loses all its digits when the mean is large.
+#include "ur_rows.h"
+
+#include <algorithm>
+
+using namespace ur;
+
+namespace {
+
+struct LnParams {
+  const void* x;
+  int64_t x_stride;
+  const void* dy;
+  int64_t dy_stride;
+  const void* w;
+  const void* b;
+  int param_dtype;
+  int64_t rows, cols;
+  float eps;
+  void* y;  // forward: y; backward: dx
+  float* mean;
+  float* rstd;
+  float* ws;      // partial results of this call
+  int64_t chunk;  // long rows: elements of a row one workgroup takes
+  int chunks;
+  int parts;      // backward: rows of partial weight sums in `ws_parts`
+  float* ws_parts;
+  void* dw;
+  void* db;
+};
+
+// parameters of kN consecutive columns as floats (1 / 0 behind the row's end or without a parameter)
+template <typename T>
+__device__ __forceinline__ void load_params(const void* p, int dtype, int64_t col, int64_t cols, float missing,
+                                            float (&out)[Elem<T>::kN]) {
+  constexpr int N = Elem<T>::kN;
+  if (p == nullptr) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) out[j] = missing;
+  } else if (dtype == UR_F32) {
+    const float* f = static_cast<const float*>(p);
+#pragma unroll
+    for (int k = 0; k < N; k += 4) {
+      const f32x4 v = load16<float>(f, col + k, cols, missing);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) out[k + j] = v[j];
+    }
+  } else {
+    const auto v = load16<T>(static_cast<const T*>(p), col, cols, (T)missing);
+#pragma unroll
+    for (int j = 0; j < N; ++j) out[j] = (float)v[j];
+  }
+}
+
+// ---- rows that fit the registers of TPR threads, NV 16-byte vectors each -------------------------------------------
+template <typename T, int TPR, int NV>
+__global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR) k_ln_fwd(const LnParams P) {
+  constexpr int N = Elem<T>::kN, kRows = TPR <= 64 ? 256 / TPR : 1;
+  __shared__ float part[2][TPR <= 64 ? 1 : TPR / 64];
+  const int t = threadIdx.x % TPR;
+  const int64_t want = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
+  const bool mine = want < P.rows;
+  const int64_t row = mine ? want : P.rows - 1;  // (idle lanes take part in the lane exchanges)
+  const T* x = static_cast<const T*>(P.x) + row * P.x_stride;
+  typename Elem<T>::Vec v[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) v[i] = load16<T>(x, (int64_t)(t + i * TPR) * N, P.cols, (T)0.0f);
+  float s[1] = {0.0f};
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j) s[0] += (float)v[i][j];
+  sum_threads<TPR, 1>(s, part[0]);
+  const float inv_d = 1.0f / (float)P.cols;
+  const float mean = s[0] * inv_d;
+  float q[1] = {0.0f};
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int64_t left = P.cols - (int64_t)(t + i * TPR) * N;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float d = (float)v[i][j] - mean;
+      if (j < left) q[0] = __builtin_fmaf(d, d, q[0]);
+    }
+  }
+  sum_threads<TPR, 1>(q, part[1]);
+  const float rstd = 1.0f / sqrtf(q[0] * inv_d + P.eps);
+  if (mine && t == 0 && P.mean) {
+    P.mean[row] = mean;
+    P.rstd[row] = rstd;
+  }
+  T* y = static_cast<T*>(P.y) + row * P.cols;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int64_t col = (int64_t)(t + i * TPR) * N;
+    if (col >= P.cols || !mine) continue;
+    float w[N], b[N];
+    load_params<T>(P.w, P.param_dtype, col, P.cols, 1.0f, w);
+    load_params<T>(P.b, P.param_dtype, col, P.cols, 0.0f, b);
+    typename Elem<T>::Vec o;
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] = (T)__builtin_fmaf(((float)v[i][j] - mean) * rstd, w[j], b[j]);
+    store16<T>(y, col, P.cols, o);
+  }
+}
+
+// Workgroups walk over the rows; a thread keeps its columns' sums of dy h and dy in registers on the way.  At the end
+// the workgroup's groups of threads are added in order and stored as one row of partial sums, which k_ln_param_sums
+// adds up: no atomics, the same result every time.
+template <typename T, int TPR, int NV>
+__global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR) k_ln_bwd(const LnParams P) {
+  constexpr int N = Elem<T>::kN, kRows = TPR <= 64 ? 256 / TPR : 1;
+  __shared__ float part[2][TPR <= 64 ? 1 : 2 * (TPR / 64)];
+  __shared__ float sums[kRows > 1 ? 2 * TPR * NV * N : 1];
+  const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  float aw[NV][N], ab[NV][N];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j) aw[i][j] = ab[i][j] = 0.0f;
+  const float inv_d = 1.0f / (float)P.cols;
+  const int64_t groups = (P.rows + kRows - 1) / kRows;
+  int flip = 0;
+  for (int64_t rg = blockIdx.x; rg < groups; rg += gridDim.x) {
+    const int64_t want = rg * kRows + sub;
+    const bool mine = want < P.rows;
+    const int64_t row = mine ? want : P.rows - 1;
+    const T* x = static_cast<const T*>(P.x) + row * P.x_stride;
+    const T* dy = static_cast<const T*>(P.dy) + row * P.dy_stride;
+    typename Elem<T>::Vec v[NV], u[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      v[i] = load16<T>(x, (int64_t)(t + i * TPR) * N, P.cols, (T)0.0f);
+      u[i] = load16<T>(dy, (int64_t)(t + i * TPR) * N, P.cols, (T)0.0f);
+    }
+    const float mean = P.mean[row], rstd = P.rstd[row];
+    float s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int64_t col = (int64_t)(t + i * TPR) * N;
+      if (col >= P.cols) continue;
+      float w[N];
+      load_params<T>(P.w, P.param_dtype, col, P.cols, 1.0f, w);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float h = ((float)v[i][j] - mean) * rstd, d = (float)u[i][j], g = d * w[j];
+        if (col + j < P.cols) {  // (a column behind the end has dy = 0, but its h may be infinite)
+          s[0] += g;
+          s[1] = __builtin_fmaf(g, h, s[1]);
+          if (mine) {
+            aw[i][j] = __builtin_fmaf(d, h, aw[i][j]);
+            ab[i][j] += d;
+          }
+        }
+      }
+    }
+    sum_threads<TPR, 2>(s, part[flip]);
+    flip ^= 1;  // (the next row's partial sums go to the other half: one barrier a row is enough)
+    if (P.y == nullptr || !mine) continue;
+    const float c1 = s[0] * inv_d, c2 = s[1] * inv_d;
+    T* dx = static_cast<T*>(P.y) + row * P.cols;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int64_t col = (int64_t)(t + i * TPR) * N;
+      if (col >= P.cols) continue;
+      float w[N];
+      load_params<T>(P.w, P.param_dtype, col, P.cols, 1.0f, w);
+      typename Elem<T>::Vec o;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float h = ((float)v[i][j] - mean) * rstd, g = (float)u[i][j] * w[j];
+        o[j] = (T)(rstd * (g - c1 - h * c2));
+      }
+      store16<T>(dx, col, P.cols, o);
+    }
+  }
+  if (P.ws_parts == nullptr) return;
+  float* out = P.ws_parts + (int64_t)blockIdx.x * 2 * P.cols;
+  if constexpr (kRows > 1) {
+    constexpr int C = TPR * NV * N;
+    for (int r = 0; r < kRows; ++r) {
+      if (r) __syncthreads();
+      if (sub == r) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            const int c = (t + i * TPR) * N + j;
+            sums[c] = r ? sums[c] + aw[i][j] : aw[i][j];
+            sums[C + c] = r ? sums[C + c] + ab[i][j] : ab[i][j];
+          }
+      }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < P.cols; c += 256) {
+      out[c] = sums[c];
+      out[P.cols + c] = sums[C + c];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int64_t col = (int64_t)(t + i * TPR) * N;
+#pragma unroll
+      for (int j = 0; j < N; j += 4) {
+        const f32x4 a = {aw[i][j], aw[i][j + 1], aw[i][j + 2], aw[i][j + 3]};
+        const f32x4 c = {ab[i][j], ab[i][j + 1], ab[i][j + 2], ab[i][j + 3]};
+        if (col + j < P.cols) {
+          store16<float>(out, col + j, P.cols, a);
+          store16<float>(out + P.cols, col + j, P.cols, c);
+        }
+      }
+    }
+  }
+}
+
+// dw, db = the sums of the partial rows: 32 columns a workgroup (one 128-byte line of a partial row), 32 groups of
+// threads over the partial rows, added in 64 bits and in a fixed order.
+__global__ void __launch_bounds__(1024) k_ln_param_sums(const LnParams P) {
+  __shared__ double acc[32][33];
+  const int c = threadIdx.x & 31, grp = threadIdx.x >> 5;
+  const int64_t col = (int64_t)blockIdx.x * 32 + c;  // 0 .. 2 D
+  double s = 0.0;
+  if (col < 2 * P.cols)
+    for (int p = grp; p < P.parts; p += 32) s += (double)P.ws_parts[(int64_t)p * 2 * P.cols + col];
+  acc[grp][c] = s;
+  __syncthreads();
+  if (grp != 0 || col >= 2 * P.cols) return;
+  double total = 0.0;
+  for (int g = 0; g < 32; ++g) total += acc[g][c];
+  if (col < P.cols) {
+    if (P.dw) store_from_float(P.dw, P.param_dtype, col, (float)total);
+  } else if (P.db) {
+    store_from_float(P.db, P.param_dtype, col - P.cols, (float)total);
+  }
+}
+
+// ---- long rows: a row is split over workgroups ----------------------------------------------------------------------
+// Forward: (1) every chunk's mean and sum of squared differences from it, (2) each chunk's workgroup merges the row's
+// chunks and writes its part.  x is read twice, the second time mostly from the caches.
+constexpr int kLongThreads = 256, kLongVecs = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(kLongThreads) k_ln_long_stats(const LnParams P) {
+  constexpr int N = Elem<T>::kN;
+  __shared__ float part[2][kLongThreads / 64];
+  const int64_t row = blockIdx.y;
+  const T* x = static_cast<const T*>(P.x) + row * P.x_stride;
+  const int64_t c0 = (int64_t)blockIdx.x * P.chunk, c1 = min(c0 + P.chunk, P.cols);
+  float n = 0.0f, mean = 0.0f, m2 = 0.0f;
+  for (int64_t base = c0; base < c1; base += kLongThreads * kLongVecs * N) {
+    typename Elem<T>::Vec v[kLongVecs];
+    float s[1] = {0.0f}, q[1] = {0.0f};
+#pragma unroll
+    for (int i = 0; i < kLongVecs; ++i) {
+      v[i] = load16<T>(x, base + (int64_t)(threadIdx.x + i * kLongThreads) * N, c1, (T)0.0f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) s[0] += (float)v[i][j];
+    }
+    sum_threads<kLongThreads, 1>(s, part[0]);
+    const float cnt = (float)min((int64_t)(kLongThreads * kLongVecs * N), c1 - base), m = s[0] / cnt;
+#pragma unroll
+    for (int i = 0; i < kLongVecs; ++i) {
+      const int64_t left = c1 - (base + (int64_t)(threadIdx.x + i * kLongThreads) * N);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float d = (float)v[i][j] - m;
+        if (j < left) q[0] = __builtin_fmaf(d, d, q[0]);
+      }
+    }
+    sum_threads<kLongThreads, 1>(q, part[1]);
+    // merge of two sets' means and squared sums
+    const float d = m - mean, total = n + cnt;
+    mean += d * (cnt / total);
+    m2 += q[0] + d * d * (n * (cnt / total));
+    n = total;
+  }
+  if (threadIdx.x == 0) {
+    P.ws[(row * P.chunks + blockIdx.x) * 2] = mean;
+    P.ws[(row * P.chunks + blockIdx.x) * 2 + 1] = m2;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kLongThreads) k_ln_long_apply(const LnParams P) {
+  constexpr int N = Elem<T>::kN;
+  const int64_t row = blockIdx.y;
+  const float* st = P.ws + row * P.chunks * 2;
+  const int lane = threadIdx.x & 63;
+  float s = 0.0f;
+  for (int i = lane; i < P.chunks; i += 64)
+    s = __builtin_fmaf(st[2 * i], (float)min(P.chunk, P.cols - i * P.chunk), s);
+  const float mean = reduce_lanes<64, OpSum>(s) / (float)P.cols;
+  float q = 0.0f;
+  for (int i = lane; i < P.chunks; i += 64) {
+    const float d = st[2 * i] - mean;
+    q += st[2 * i + 1] + d * d * (float)min(P.chunk, P.cols - i * P.chunk);
+  }
+  const float rstd = 1.0f / sqrtf(reduce_lanes<64, OpSum>(q) / (float)P.cols + P.eps);
+  if (blockIdx.x == 0 && threadIdx.x == 0 && P.mean) {
+    P.mean[row] = mean;
+    P.rstd[row] = rstd;
+  }
+  const T* x = static_cast<const T*>(P.x) + row * P.x_stride;
+  T* y = static_cast<T*>(P.y) + row * P.cols;
+  const int64_t c0 = (int64_t)blockIdx.x * P.chunk, c1 = min(c0 + P.chunk, P.cols);
+  for (int64_t col = c0 + (int64_t)threadIdx.x * N; col < c1; col += kLongThreads * N) {
+    const auto v = load16<T>(x, col, c1, (T)0.0f);
+    float w[N], b[N];
+    load_params<T>(P.w, P.param_dtype, col, P.cols, 1.0f, w);
+    load_params<T>(P.b, P.param_dtype, col, P.cols, 0.0f, b);
+    typename Elem<T>::Vec o;
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] = (T)__builtin_fmaf(((float)v[j] - mean) * rstd, w[j], b[j]);
+    store16<T>(y, col, c1, o);
+  }
+}
+
+// Backward: (1) every chunk's sums of g and g h, (2) a workgroup takes a strip of columns through a range of rows: dx, and
+// its columns' partial weight sums; (3) k_ln_param_sums.
+template <typename T>
+__global__ void __launch_bounds__(kLongThreads) k_ln_long_bwd_sums(const LnParams P) {
+  constexpr int N = Elem<T>::kN;
+  __shared__ float part[2 * (kLongThreads / 64)];
+  const int64_t row = blockIdx.y;
+  const T* x = static_cast<const T*>(P.x) + row * P.x_stride;
+  const T* dy = static_cast<const T*>(P.dy) + row * P.dy_stride;
+  const float mean = P.mean[row], rstd = P.rstd[row];
+  const int64_t c0 = (int64_t)blockIdx.x * P.chunk, c1 = min(c0 + P.chunk, P.cols);
+  float s[2] = {0.0f, 0.0f};
+  for (int64_t col = c0 + (int64_t)threadIdx.x * N; col < c1; col += kLongThreads * N) {
+    const auto v = load16<T>(x, col, c1, (T)0.0f), u = load16<T>(dy, col, c1, (T)0.0f);
+    float w[N];
+    load_params<T>(P.w, P.param_dtype, col, P.cols, 1.0f, w);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float g = (float)u[j] * w[j];
+      if (col + j < c1) {
+        s[0] += g;
+        s[1] = __builtin_fmaf(g, ((float)v[j] - mean) * rstd, s[1]);
+      }
+    }
+  }
+  sum_threads<kLongThreads, 2>(s, part);
+  if (threadIdx.x == 0) {
+    P.ws[(row * P.chunks + blockIdx.x) * 2] = s[0];
+    P.ws[(row * P.chunks + blockIdx.x) * 2 + 1] = s[1];
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kLongThreads) k_ln_long_bwd_apply(const LnParams P) {
+  constexpr int N = Elem<T>::kN;
+  const int lane = threadIdx.x & 63;
+  const int64_t col = ((int64_t)blockIdx.x * kLongThreads + threadIdx.x) * N;
+  const bool inside = col < P.cols;
+  float w[N], aw[N], ab[N];
+  load_params<T>(P.w, P.param_dtype, inside ? col : 0, P.cols, 1.0f, w);
+#pragma unroll
+  for (int j = 0; j < N; ++j) aw[j] = ab[j] = 0.0f;
+  for (int64_t row = blockIdx.y; row < P.rows; row += gridDim.y) {
+    const float* st = P.ws + row * P.chunks * 2;
+    float s0 = 0.0f, s1 = 0.0f;
+    for (int i = lane; i < P.chunks; i += 64) {
+      s0 += st[2 * i];
+      s1 += st[2 * i + 1];
+    }
+    const float c1 = reduce_lanes<64, OpSum>(s0) / (float)P.cols, c2 = reduce_lanes<64, OpSum>(s1) / (float)P.cols;
+    if (!inside) continue;
+    const float mean = P.mean[row], rstd = P.rstd[row];
+    const auto v = load16<T>(static_cast<const T*>(P.x) + row * P.x_stride, col, P.cols, (T)0.0f);
+    const auto u = load16<T>(static_cast<const T*>(P.dy) + row * P.dy_stride, col, P.cols, (T)0.0f);
+    typename Elem<T>::Vec o;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float h = ((float)v[j] - mean) * rstd, d = (float)u[j];
+      aw[j] = __builtin_fmaf(d, h, aw[j]);
+      ab[j] += d;
+      o[j] = (T)(rstd * (d * w[j] - c1 - h * c2));
+    }
+    if (P.y) store16<T>(static_cast<T*>(P.y) + row * P.cols, col, P.cols, o);
+  }
+  if (P.ws_parts == nullptr || !inside) return;
+  float* out = P.ws_parts + (int64_t)blockIdx.y * 2 * P.cols;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (col + j < P.cols) {
+      out[col + j] = aw[j];
+      out[P.cols + col + j] = ab[j];
+    }
+}
+
+// ---- which kernel a call takes ---------------------------------------------------------------------------------------
+struct LnPlan {
+  int tpr, nv;      // threads a row and vectors a thread; tpr == 0: long rows
+  int64_t chunk;    // long rows
+  int chunks;
+  int grid;         // backward: workgroups (register rows) or row ranges (long rows) = rows of partial sums
+  int64_t ws_stats, ws_parts;  // floats
+};
+
+LnPlan ln_plan(int64_t rows, int64_t cols, int dtype, bool backward) {
+  LnPlan p{};
+  const int n = 16 / dtype_bytes(dtype);
+  const int64_t vecs = ceil_div(cols, n);
+  struct Shape { int tpr, nv; };
+  static constexpr Shape kFwd[] = {{16, 2}, {64, 1}, {64, 2}, {64, 4}, {64, 8}, {256, 4}, {256, 8}, {1024, 4}, {1024, 8}};
+  static constexpr Shape kBwd[] = {{16, 2}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {512, 4}};
+  const Shape* shapes = backward ? kBwd : kFwd;
+  const int count = backward ? (int)(sizeof(kBwd) / sizeof(Shape)) : (int)(sizeof(kFwd) / sizeof(Shape));
+  for (int i = 0; i < count; ++i)
+    if (vecs <= (int64_t)shapes[i].tpr * shapes[i].nv) {
+      p.tpr = shapes[i].tpr;
+      p.nv = shapes[i].nv;
+      break;
+    }
+  if (p.tpr) {
+    const int per = p.tpr <= 64 ? 256 / p.tpr : 1;
+    p.grid = (int)std::min<int64_t>(ceil_div(rows, per), 1024);
+    p.ws_parts = backward ? (int64_t)p.grid * 2 * cols : 0;
+    return p;
+  }
+  const int64_t step = (int64_t)kLongThreads * kLongVecs * n;
+  p.chunk = ceil_div(ceil_div(cols, 1024), step) * step;  // at most 1024 chunks a row
+  p.chunks = (int)ceil_div(cols, p.chunk);
+  p.ws_stats = rows * p.chunks * 2;
+  const int64_t strips = ceil_div(cols, (int64_t)kLongThreads * n);
+  p.grid = (int)std::min<int64_t>(rows, std::max<int64_t>(1, 2048 / strips));
+  p.ws_parts = backward ? (int64_t)p.grid * 2 * cols : 0;
+  return p;
+}
+
+int check_common(const void* x, int64_t x_stride, int dtype, int param_dtype, int64_t rows, int64_t cols) {
+  if (!x) return set_error(UR_ERR_INVALID_ARG, "null input pointer");
+  if (!known_dtype(dtype)) return set_error(UR_ERR_INVALID_ARG, "bad dtype %d", dtype);
+  if (param_dtype != dtype && param_dtype != UR_F32)
+    return set_error(UR_ERR_INVALID_ARG, "parameters must have the input's type or fp32");
+  if (rows <= 0 || cols <= 0) return set_error(UR_ERR_INVALID_ARG, "rows and cols must be positive");
+  if (rows > 0x7fffffff || cols > 0x7fffffff) return set_error(UR_ERR_UNSUPPORTED, "rows and cols must be below 2^31");
+  if (x_stride < cols && rows > 1) return set_error(UR_ERR_INVALID_ARG, "row stride below the row length");
+  return UR_OK;
+}
+
+template <typename T>
+int launch_fwd(const LnPlan& p, const LnParams& P, hipStream_t st) {
+  if (p.tpr == 0) {
+    for (int64_t r0 = 0; r0 < P.rows; r0 += 65535) {  // (the grid's second dimension holds 65535 rows)
+      LnParams Q = P;
+      Q.rows = std::min<int64_t>(65535, P.rows - r0);
+      Q.x = static_cast<const T*>(P.x) + r0 * P.x_stride;
+      Q.y = static_cast<T*>(P.y) + r0 * P.cols;
+      Q.mean = P.mean ? P.mean + r0 : nullptr;
+      Q.rstd = P.rstd ? P.rstd + r0 : nullptr;
+      Q.ws = P.ws + r0 * P.chunks * 2;
+      const dim3 grid(P.chunks, (unsigned)Q.rows);
+      k_ln_long_stats<T><<<grid, kLongThreads, 0, st>>>(Q);
+      k_ln_long_apply<T><<<grid, kLongThreads, 0, st>>>(Q);
+    }
+    return launch_status("ur_layer_norm_forward");
+  }
+  const int per = p.tpr <= 64 ? 256 / p.tpr : 1;
+  const dim3 grid((unsigned)ceil_div(P.rows, per));
+#define UR_LN(TPR, NV) \
+  if (p.tpr == TPR && p.nv == NV) k_ln_fwd<T, TPR, NV><<<grid, TPR <= 64 ? 256 : TPR, 0, st>>>(P);
+  UR_LN(16, 2) UR_LN(64, 1) UR_LN(64, 2) UR_LN(64, 4) UR_LN(64, 8) UR_LN(256, 4) UR_LN(256, 8) UR_LN(1024, 4)
+  UR_LN(1024, 8)
+#undef UR_LN
+  return launch_status("ur_layer_norm_forward");
+}
+
+template <typename T>
+int launch_bwd(const LnPlan& p, const LnParams& P, hipStream_t st) {
+  if (p.tpr == 0) {
+    for (int64_t r0 = 0; r0 < P.rows; r0 += 65535) {
+      LnParams Q = P;
+      Q.rows = std::min<int64_t>(65535, P.rows - r0);
+      Q.x = static_cast<const T*>(P.x) + r0 * P.x_stride;
+      Q.dy = static_cast<const T*>(P.dy) + r0 * P.dy_stride;
+      Q.mean = P.mean + r0;
+      Q.rstd = P.rstd + r0;
+      Q.ws = P.ws + r0 * P.chunks * 2;
+      k_ln_long_bwd_sums<T><<<dim3(P.chunks, (unsigned)Q.rows), kLongThreads, 0, st>>>(Q);
+    }
+    const unsigned strips = (unsigned)ceil_div(P.cols, (int64_t)kLongThreads * Elem<T>::kN);
+    k_ln_long_bwd_apply<T><<<dim3(strips, p.grid), kLongThreads, 0, st>>>(P);
+  } else {
+    const dim3 grid(p.grid);
+#define UR_LN(TPR, NV) \
+  if (p.tpr == TPR && p.nv == NV) k_ln_bwd<T, TPR, NV><<<grid, TPR <= 64 ? 256 : TPR, 0, st>>>(P);
+    UR_LN(16, 2) UR_LN(64, 1) UR_LN(64, 2) UR_LN(64, 4) UR_LN(256, 2) UR_LN(256, 4) UR_LN(512, 4)
+#undef UR_LN
+  }
+  if (P.ws_parts) k_ln_param_sums<<<dim3((unsigned)ceil_div(2 * P.cols, 32)), 1024, 0, st>>>(P);
+  return launch_status("ur_layer_norm_backward");
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t ur_layer_norm_workspace_bytes(int64_t rows, int64_t cols, int dtype, int backward) {
+  if (!known_dtype(dtype)) return set_error(UR_ERR_INVALID_ARG, "bad dtype %d", dtype);
+  if (rows <= 0 || cols <= 0 || rows > 0x7fffffff || cols > 0x7fffffff)
+    return set_error(UR_ERR_INVALID_ARG, "rows and cols must be positive and below 2^31");
+  const LnPlan p = ln_plan(rows, cols, dtype, backward != 0);
+  return (p.ws_stats + p.ws_parts) * 4;
+}
+
+int ur_layer_norm_forward(const void* x, int64_t x_row_stride, const void* weight, const void* bias, int dtype,
+                          int param_dtype, int64_t rows, int64_t cols, float eps, void* y, float* mean, float* rstd,
+                          void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_common(x, x_row_stride, dtype, param_dtype, rows, cols)) return rc;
+  if (!y) return set_error(UR_ERR_INVALID_ARG, "null output pointer");
+  if ((mean == nullptr) != (rstd == nullptr)) return set_error(UR_ERR_INVALID_ARG, "mean and rstd go together");
+  if (!(eps >= 0.0f)) return set_error(UR_ERR_INVALID_ARG, "eps must not be negative");
+  const LnPlan p = ln_plan(rows, cols, dtype, false);
+  const size_t need = (size_t)(p.ws_stats + p.ws_parts) * 4;
+  if (workspace_bytes < need || (need && !workspace))
+    return set_error(UR_ERR_WORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, need);
+  LnParams P{};
+  P.x = x; P.x_stride = x_row_stride; P.w = weight; P.b = bias; P.param_dtype = param_dtype;
+  P.rows = rows; P.cols = cols; P.eps = eps; P.y = y; P.mean = mean; P.rstd = rstd;
+  P.ws = static_cast<float*>(workspace); P.chunk = p.chunk; P.chunks = p.chunks;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == UR_F32) return launch_fwd<float>(p, P, st);
+  if (dtype == UR_F16) return launch_fwd<_Float16>(p, P, st);
+  return launch_fwd<__bf16>(p, P, st);
+}
+
+int ur_layer_norm_backward(const void* grad_y, int64_t grad_row_stride, const void* x, int64_t x_row_stride,
+                           const void* weight, const float* mean, const float* rstd, int dtype, int param_dtype,
+                           int64_t rows, int64_t cols, void* grad_x, void* grad_weight, void* grad_bias,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_common(x, x_row_stride, dtype, param_dtype, rows, cols)) return rc;
+  if (!grad_y || !mean || !rstd) return set_error(UR_ERR_INVALID_ARG, "null input pointer");
+  if (grad_row_stride < cols && rows > 1) return set_error(UR_ERR_INVALID_ARG, "row stride below the row length");
+  if (!grad_x && !grad_weight && !grad_bias) return set_error(UR_ERR_INVALID_ARG, "no gradient asked for");
+  const LnPlan p = ln_plan(rows, cols, dtype, true);
+  const size_t need = (size_t)(p.ws_stats + p.ws_parts) * 4;
+  if (workspace_bytes < need || !workspace)
+    return set_error(UR_ERR_WORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, need);
+  LnParams P{};
+  P.x = x; P.x_stride = x_row_stride; P.dy = grad_y; P.dy_stride = grad_row_stride; P.w = weight;
+  P.param_dtype = param_dtype; P.rows = rows; P.cols = cols; P.y = grad_x;
+  P.mean = const_cast<float*>(mean); P.rstd = const_cast<float*>(rstd);
+  P.ws = static_cast<float*>(workspace); P.chunk = p.chunk; P.chunks = p.chunks;
+  P.parts = p.grid; P.ws_parts = (grad_weight || grad_bias) ? P.ws + p.ws_stats : nullptr;
+  P.dw = grad_weight; P.db = grad_bias;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == UR_F32) return launch_bwd<float>(p, P, st);
+  if (dtype == UR_F16) return launch_bwd<_Float16>(p, P, st);
+  return launch_bwd<__bf16>(p, P, st);
+}
+
+}  // extern "C"

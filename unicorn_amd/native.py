@@ -54,6 +54,10 @@ _SIGNATURES = {
                                        _i, _vp, _vp, _vp, _vp]),
     "ur_shade_blend_backward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _f, _vp, _vp, _i,
                                      _vp, _vp, _vp, _vp]),
+    "ur_layer_norm_workspace_bytes": (_i64, [_i64, _i64, _i, _i]),
+    "ur_layer_norm_forward": (_i, [_vp, _i64, _vp, _vp, _i, _i, _i64, _i64, _f, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ur_layer_norm_backward": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i, _i, _i64, _i64, _vp, _vp, _vp, _vp, _sz,
+                                    _vp]),
 }
 
 
@@ -602,3 +606,88 @@ def selftest_division(n, seed=0, device="cuda"):
     with _on(out):
         _check(lib().ur_selftest_division(int(n), int(seed), _ptr(out), _stream(out)), "ur_selftest_division")
     return int(out.item())
+
+
+# ---- operators of the networks around the renderer (rows of fp32 / fp16 / bf16) -------------------------------------
+F32, F16, BF16 = 0, 1, 2  # UR_F32, UR_F16, UR_BF16
+_DTYPE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+
+
+def dtype_code(t, what="tensor"):
+    code = _DTYPE.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
+    return code
+
+
+def same_device(t, *others):
+    """`t` lives on a GPU and so do the others, on the same one"""
+    if not t.is_cuda:
+        _ptr(t)
+    for o in others:
+        if o is not None and o.device != t.device:
+            raise ValueError(f"tensors must be on one device: {t.device} and {o.device}")
+
+
+def rows_of(t):
+    """(tensor, rows, row stride) of a tensor read as rows of its last dimension: as it lies where its rows are dense and
+    evenly spaced without overlap (any stride between them), a contiguous copy otherwise"""
+    D = t.shape[-1]
+    if t.is_contiguous():
+        return t, t.numel() // D if D else 0, D
+    if D == 1 or t.stride(-1) == 1:
+        flat = t
+        if t.dim() != 2:
+            try:
+                flat = t.view(-1, D)
+            except RuntimeError:
+                flat = None
+        if flat is not None and (flat.shape[0] <= 1 or flat.stride(0) >= D):
+            return flat, flat.shape[0], max(flat.stride(0), D)
+    t = t.contiguous()
+    return t, t.numel() // D if D else 0, D
+
+
+def _ws(nbytes, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def layer_norm_forward(x, weight, bias, eps, need_stats):
+    """x (..., D) -> y (x's shape, contiguous), mean, rstd (f32, one per row; None unless asked for)"""
+    same_device(x, weight, bias)
+    code = dtype_code(x)
+    pcode = code if weight is None and bias is None else dtype_code(weight if weight is not None else bias)
+    x, M, stride = rows_of(x)
+    D = x.shape[-1]
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty((2, M), dtype=torch.float32, device=x.device) if need_stats else None
+    if M:
+        n = _sized("ur_layer_norm_workspace_bytes", M, D, code, 0)
+        ws = _ws(n, x.device)
+        p = stats.data_ptr() if need_stats else None
+        _call("ur_layer_norm_forward", x, x.data_ptr(), stride, _ptr(weight, None, True), _ptr(bias, None, True), code,
+              pcode, M, D, eps, y.data_ptr(), p, p + 4 * M if need_stats else None,
+              ws.data_ptr() if n else None, n, _stream(x))
+    return y, stats
+
+
+def layer_norm_backward(grad_y, x, weight, param_dtype, stats, need_x, need_weight, need_bias):
+    """-> grad_x (x's shape), grad_weight, grad_bias (D); None where not asked for"""
+    code = dtype_code(x)
+    grad_y, M, gstride = rows_of(grad_y)
+    x, _, stride = rows_of(x)
+    D = x.shape[-1]
+    dev = x.device
+    if not M:
+        zeros = lambda need: torch.zeros(D, dtype=param_dtype, device=dev) if need else None
+        return (torch.empty_like(x) if need_x else None), zeros(need_weight), zeros(need_bias)
+    gx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+    gw = torch.empty(D, dtype=param_dtype, device=dev) if need_weight else None
+    gb = torch.empty(D, dtype=param_dtype, device=dev) if need_bias else None
+    n = _sized("ur_layer_norm_workspace_bytes", M, D, code, 1)
+    ws = _ws(n, dev)
+    p = stats.data_ptr()
+    _call("ur_layer_norm_backward", x, grad_y.data_ptr(), gstride, x.data_ptr(), stride, _ptr(weight, None, True), p,
+          p + 4 * M, code, _DTYPE[param_dtype] if param_dtype is not None else code, M, D, _ptr(gx, None, True),
+          _ptr(gw, None, True), _ptr(gb, None, True), ws.data_ptr() if n else None, n, _stream(x))
+    return gx, gw, gb
