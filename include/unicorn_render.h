@@ -321,6 +321,34 @@ int ur_layer_norm_backward(const void* grad_y, int64_t grad_row_stride, const vo
                            int64_t rows, int64_t cols, void* grad_x, void* grad_weight, void* grad_bias,
                            void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Routing: which `top_k` of a row's candidates are taken (rendered, computed), with which weights, and how often each
+ * candidate was taken over all rows.
+ *   s = softmax(l) or sigmoid(l) ; c = s + bias (fp32, `cands`, may be NULL: then c's order is l's) ;
+ *   groups: consecutive runs of cands / groups candidates; a group's value is its largest c or the sum of its two largest;
+ *   the `top_groups` best groups stay ; indices = the top_k largest c left, largest first ; ties: the lowest index ;
+ *   weights = scale * s / (sum of the chosen s) (renormalize != 0) or scale * s.
+ *   The order is that of the 64-bit values of c.  A candidate with l = -inf or bias = -inf is not eligible; a slot that no
+ *   eligible candidate is left for holds index -1 and weight 0.  NaN counts as the largest value and makes weights NaN.
+ *   logits (rows, cands), row i at logits + i * row_stride ; weights fp32, indices int64 (rows, top_k) ; counts int32 (cands).
+ *   At most 1024 candidates, 64 choices, 64 groups (UR_ERR_UNSUPPORTED beyond).
+ * Backward: grad_weights fp32 (rows, top_k), and the forward's weights and indices -> grad_logits (rows, cands) of the
+ *   logits' type; the bias gets none.
+ * workspace: ur_route_workspace_bytes(rows, cands) of uninitialised memory (0 is possible); negative = error.
+ */
+#define UR_SCORE_SOFTMAX 0
+#define UR_SCORE_SIGMOID 1
+#define UR_GROUP_MAX 0
+#define UR_GROUP_TOP2 1
+int64_t ur_route_workspace_bytes(int64_t rows, int cands);
+int ur_route_forward(const void* logits, int64_t row_stride, int dtype, const float* bias, int64_t rows, int cands,
+                     int top_k, int score, int groups, int top_groups, int group_score, int renormalize, float scale,
+                     float* weights, int64_t* indices, int32_t* counts, void* workspace, size_t workspace_bytes,
+                     void* stream);
+int ur_route_backward(const float* grad_weights, const void* logits, int64_t row_stride, int dtype, int64_t rows,
+                      int cands, const float* weights, const int64_t* indices, int top_k, int score,
+                      int renormalize, float scale, void* grad_logits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

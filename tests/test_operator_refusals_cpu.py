@@ -78,3 +78,47 @@ def test_layer_norm_workspace_sizes():
             n = size(M, D, dt, 1)
             assert n >= 2 * D * 4 and n % 4 == 0                        # at least one row of partial sums
             assert size(M, D, dt, 0) <= n
+
+
+def test_routing_python_checks():
+    from unicorn_amd.routing import route_candidates
+    l = torch.randn(4, 12)
+    cases = [("GPU", (l, 2), {}), ("GPU", (l.clone().requires_grad_(True), 2), {}),
+             ("float32, float16", (l.double(), 2), {}), ("float32, float16", (l.long(), 2), {}),
+             ("at least 1", (torch.empty(3, 0), 1), {}), ("at least 1", (torch.tensor(1.0), 1), {}),
+             ("score must", (l, 2), {"score": "relu"}), ("group_score must", (l, 2), {"group_score": "sum"}),
+             ("groups must divide", (l, 2), {"groups": 5}), ("groups must divide", (l, 2), {"groups": 0}),
+             ("top_groups must", (l, 2), {"groups": 3, "top_groups": 4}), ("top_groups must", (l, 2), {"top_groups": 0}),
+             ("top_k must", (l, 0), {}), ("top_k must", (l, 13), {}), ("top_k must", (l, 5), {"groups": 3, "top_groups": 1}),
+             ("finite", (l, 2), {"scale": float("inf")}), ("finite", (l, 2), {"scale": float("nan")}),
+             ("bias must", (l, 2), {"bias": torch.zeros(11)}), ("bias must", (l, 2), {"bias": torch.zeros(12).half()}),
+             ("bias must", (l, 2), {"bias": torch.zeros(1, 12)})]
+    for match, args, kw in cases:
+        with pytest.raises(ValueError, match=match):
+            route_candidates(*args, **kw)
+    for args, kw in (((torch.randn(2, 1025), 2), {}), ((torch.randn(2, 100), 65), {}),
+                     ((torch.randn(2, 130), 2), {"groups": 65, "top_groups": 65})):
+        with pytest.raises(NotImplementedError, match="at most"):
+            route_candidates(*args, **kw)
+
+
+def test_routing_entry_point_checks():
+    def fwd(l=FAKE, stride=12, dt=0, M=1, E=12, k=2, score=0, G=1, tg=1, gs=0, scale=1.0, w=FAKE, i=FAKE, c=FAKE, ws=None, n=0):
+        return refused("ur_route_forward", l, stride, dt, None, M, E, k, score, G, tg, gs, 1, scale, w, i, c, ws, n, None)
+    for kw in ({"l": None}, {"w": None}, {"i": None}, {"c": None}, {"dt": 3}, {"M": 0}, {"E": 0}, {"k": 0}, {"k": 13},
+               {"score": 2}, {"G": 5}, {"G": 0}, {"G": 3, "tg": 4}, {"tg": 0}, {"G": 3, "tg": 1, "k": 5}, {"gs": 2},
+               {"scale": float("nan")}, {"scale": float("inf")}, {"stride": 11, "M": 2}):
+        assert fwd(**kw)[0] == -1, kw
+    for kw in ({"E": 1025, "stride": 1025}, {"E": 128, "stride": 128, "k": 65}, {"E": 130, "stride": 130, "G": 65, "tg": 65},
+               {"M": 1 << 31}):
+        assert fwd(**kw)[0] == -2, kw
+    assert fwd(M=1000)[0] == -4
+
+    def bwd(g=FAKE, l=FAKE, dt=0, M=1, E=12, w=FAKE, i=FAKE, k=2, score=0, scale=1.0, out=FAKE):
+        return refused("ur_route_backward", g, l, 12, dt, M, E, w, i, k, score, 1, scale, out, None)
+    for kw in ({"g": None}, {"l": None}, {"w": None}, {"i": None}, {"out": None}, {"dt": -1}, {"M": 0}, {"k": 13}, {"score": 5},
+               {"scale": float("inf")}):
+        assert bwd(**kw)[0] == -1, kw
+    for args in ((0, 4), (4, 0), (1 << 31, 4), (4, 1025)):
+        assert refused("ur_route_workspace_bytes", *args)[0] == -1
+    assert native.lib().ur_route_workspace_bytes(1, 12) == 0

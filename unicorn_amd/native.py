@@ -58,6 +58,9 @@ _SIGNATURES = {
     "ur_layer_norm_forward": (_i, [_vp, _i64, _vp, _vp, _i, _i, _i64, _i64, _f, _vp, _vp, _vp, _vp, _sz, _vp]),
     "ur_layer_norm_backward": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i, _i, _i64, _i64, _vp, _vp, _vp, _vp, _sz,
                                     _vp]),
+    "ur_route_workspace_bytes": (_i64, [_i64, _i]),
+    "ur_route_forward": (_i, [_vp, _i64, _i, _vp, _i64, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ur_route_backward": (_i, [_vp, _vp, _i64, _i, _i64, _i, _vp, _vp, _i, _i, _i, _f, _vp, _vp]),
 }
 
 
@@ -691,3 +694,35 @@ def layer_norm_backward(grad_y, x, weight, param_dtype, stats, need_x, need_weig
           p + 4 * M, code, _DTYPE[param_dtype] if param_dtype is not None else code, M, D, _ptr(gx, None, True),
           _ptr(gw, None, True), _ptr(gb, None, True), ws.data_ptr() if n else None, n, _stream(x))
     return gx, gw, gb
+
+
+def route_forward(logits, bias, top_k, score, groups, top_groups, group_score, renormalize, scale):
+    """logits (..., E) -> weights f32 (..., k), indices i64 (..., k), counts i32 (E)"""
+    same_device(logits, bias)
+    code = dtype_code(logits)
+    x, M, stride = rows_of(logits)
+    dev, E = x.device, x.shape[-1]
+    shape = logits.shape[:-1] + (top_k,)
+    weights = torch.empty(shape, dtype=torch.float32, device=dev)
+    indices = torch.empty(shape, dtype=torch.int64, device=dev)
+    if not M:
+        return weights, indices, torch.zeros(E, dtype=torch.int32, device=dev)
+    counts = torch.empty(E, dtype=torch.int32, device=dev)
+    n = _sized("ur_route_workspace_bytes", M, E)
+    ws = _ws(n, dev)
+    _call("ur_route_forward", x, x.data_ptr(), stride, code, _ptr(bias, torch.float32, True), M, E, top_k, score, groups,
+          top_groups, group_score, renormalize, scale, weights.data_ptr(), indices.data_ptr(), counts.data_ptr(),
+          ws.data_ptr() if n else None, n, _stream(x))
+    return weights, indices, counts
+
+
+def route_backward(grad_weights, logits, weights, indices, score, renormalize, scale):
+    """-> grad of logits (their shape and type)"""
+    code = dtype_code(logits)
+    x, M, stride = rows_of(logits)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=x.device)
+    if M:
+        _call("ur_route_backward", x, _ptr(grad_weights.contiguous(), torch.float32), x.data_ptr(), stride, code, M,
+              x.shape[-1], _ptr(weights, torch.float32), _ptr(indices, torch.int64), indices.shape[-1], score, renormalize,
+              scale, grad.data_ptr(), _stream(x))
+    return grad
