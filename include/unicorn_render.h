@@ -349,6 +349,35 @@ int ur_route_backward(const float* grad_weights, const void* logits, int64_t row
                       int cands, const float* weights, const int64_t* indices, int top_k, int score,
                       int renormalize, float scale, void* grad_logits, void* stream);
 
+/*
+ * Distillation from a teacher's top logits: the divergence of the student's distribution over all `cols` classes from the
+ * teacher's over the `top` classes whose logits are known.
+ *   p = softmax(t / T) over the row's filled slots ; q = softmax(z / T) over cols ;
+ *   loss_row = T^2 * sum_j p_j (log p_j - log q[index_j]) ; grad z_v = T * g * (q_v - sum over {j: index_j = v} of p_j)
+ *   logits z (rows, cols), row i at logits + i * row_stride ; teacher t (rows, top) of teacher_dtype and index (rows, top) of
+ *   index_bytes = 4 or 8 (int32 / int64), contiguous.  A negative index is an empty slot; several slots may name one class; a
+ *   row whose slots are all empty (or have t = -inf) has no teacher: loss 0, gradient 0.  An index of cols or more makes
+ *   the row's loss and gradient NaN.
+ *   reduction: UR_REDUCE_NONE: loss (rows) ; UR_REDUCE_SUM, UR_REDUCE_MEAN: one value, the mean over the rows that have a
+ *   teacher (0 if none has).
+ *   stats: 2 * rows + 1 floats kept for the backward, or NULL when there will be none.
+ * Backward: grad_loss fp32: one value, or (rows) with the stride grad_stride (elements, 0 allowed) for UR_REDUCE_NONE ->
+ *   grad_logits (rows, cols) of the logits' type.
+ * workspace: ur_distill_workspace_bytes(rows, cols, dtype, reduction) of uninitialised memory (0 is possible); negative = error.
+ * At most 1024 slots (UR_ERR_UNSUPPORTED beyond).
+ */
+#define UR_REDUCE_NONE 0
+#define UR_REDUCE_SUM 1
+#define UR_REDUCE_MEAN 2
+int64_t ur_distill_workspace_bytes(int64_t rows, int64_t cols, int dtype, int reduction);
+int ur_distill_forward(const void* logits, int64_t row_stride, int dtype, int64_t rows, int64_t cols, const void* teacher,
+                       int teacher_dtype, const void* index, int index_bytes, int top, float temperature, int reduction,
+                       float* loss, float* stats, void* workspace, size_t workspace_bytes, void* stream);
+int ur_distill_backward(const float* grad_loss, int64_t grad_stride, const void* logits, int64_t row_stride, int dtype,
+                        int64_t rows, int64_t cols, const void* teacher, int teacher_dtype, const void* index,
+                        int index_bytes, int top, float temperature, int reduction, const float* stats,
+                        void* grad_logits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -122,3 +122,39 @@ def test_routing_entry_point_checks():
     for args in ((0, 4), (4, 0), (1 << 31, 4), (4, 1025)):
         assert refused("ur_route_workspace_bytes", *args)[0] == -1
     assert native.lib().ur_route_workspace_bytes(1, 12) == 0
+
+
+def test_distillation_python_checks():
+    from unicorn_amd.distillation import distill_top_logits
+    z, t, i = torch.randn(4, 12), torch.randn(4, 3), torch.zeros(4, 3, dtype=torch.int64)
+    cases = [("GPU", (z, t, i), {}), ("GPU", (z.clone().requires_grad_(True), t, i), {}),
+             ("logits must be float32", (z.double(), t, i), {}), ("teacher_logits must be float32", (z, t.double(), i), {}),
+             ("int32 or int64", (z, t, i.float()), {}), ("int32 or int64", (z, t, i.short()), {}),
+             ("at least 1", (torch.empty(4, 0), t, i), {}), ("at least 1", (torch.tensor(1.0), t, i), {}),
+             ("must have shape", (z, t[:3], i), {}), ("must have shape", (z, t[:3], i[:3]), {}),
+             ("must have shape", (z, t[:, :0], i[:, :0]), {}), ("must have shape", (z, t[0], i[0]), {}),
+             ("must have shape", (z, t[None], i[None]), {}), ("reduction must", (z, t, i), {"reduction": "max"})]
+    cases += [("temperature", (z, t, i), {"temperature": v}) for v in (0.0, -1.0, float("inf"), float("nan"), 1e-40)]
+    for match, args, kw in cases:
+        with pytest.raises(ValueError, match=match):
+            distill_top_logits(*args, **kw)
+    with pytest.raises(NotImplementedError, match="at most 1024"):
+        distill_top_logits(z, torch.randn(4, 1025), torch.zeros(4, 1025, dtype=torch.int64))
+
+
+def test_distillation_entry_point_checks():
+    def fwd(z=FAKE, stride=12, dt=0, M=2, V=12, t=FAKE, tdt=0, i=FAKE, ib=8, k=3, T=1.0, red=0, loss=FAKE, ws=None, n=0):
+        return refused("ur_distill_forward", z, stride, dt, M, V, t, tdt, i, ib, k, T, red, loss, None, ws, n, None)
+
+    def bwd(g=FAKE, z=FAKE, stride=12, dt=0, M=2, V=12, t=FAKE, tdt=0, i=FAKE, ib=8, k=3, T=1.0, red=0, stats=FAKE, out=FAKE):
+        return refused("ur_distill_backward", g, 1, z, stride, dt, M, V, t, tdt, i, ib, k, T, red, stats, out, None)
+    both = ({"z": None}, {"t": None}, {"i": None}, {"dt": 3}, {"tdt": -1}, {"ib": 2}, {"M": 0}, {"V": 0}, {"k": 0},
+            {"stride": 11}, {"T": 0.0}, {"T": -1.0}, {"T": float("nan")}, {"T": float("inf")}, {"T": 1e-45}, {"red": 3})
+    for kw in both:
+        assert fwd(**kw)[0] == -1 and bwd(**kw)[0] == -1, kw
+    for kw in ({"k": 1025}, {"M": 1 << 31}, {"V": 1 << 31, "stride": 1 << 31}):
+        assert fwd(**kw)[0] == -2 and bwd(**kw)[0] == -2, kw
+    assert fwd(loss=None)[0] == -1 and bwd(g=None)[0] == -1 and bwd(stats=None)[0] == -1 and bwd(out=None)[0] == -1
+    assert fwd(red=2)[0] == -4 and fwd(red=1, ws=FAKE, n=8)[0] == -4
+    for args in ((0, 4, 0, 0), (4, 0, 0, 0), (1 << 31, 4, 0, 0), (4, 4, 3, 0)):
+        assert refused("ur_distill_workspace_bytes", *args)[0] == -1

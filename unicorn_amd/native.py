@@ -58,6 +58,9 @@ _SIGNATURES = {
     "ur_layer_norm_forward": (_i, [_vp, _i64, _vp, _vp, _i, _i, _i64, _i64, _f, _vp, _vp, _vp, _vp, _sz, _vp]),
     "ur_layer_norm_backward": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i, _i, _i64, _i64, _vp, _vp, _vp, _vp, _sz,
                                     _vp]),
+    "ur_distill_workspace_bytes": (_i64, [_i64, _i64, _i, _i]),
+    "ur_distill_forward": (_i, [_vp, _i64, _i, _i64, _i64, _vp, _i, _vp, _i, _i, _f, _i, _vp, _vp, _vp, _sz, _vp]),
+    "ur_distill_backward": (_i, [_vp, _i64, _vp, _i64, _i, _i64, _i64, _vp, _i, _vp, _i, _i, _f, _i, _vp, _vp, _vp]),
     "ur_route_workspace_bytes": (_i64, [_i64, _i]),
     "ur_route_forward": (_i, [_vp, _i64, _i, _vp, _i64, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _vp, _vp, _vp, _sz, _vp]),
     "ur_route_backward": (_i, [_vp, _vp, _i64, _i, _i64, _i, _vp, _vp, _i, _i, _i, _f, _vp, _vp]),
@@ -725,4 +728,44 @@ def route_backward(grad_weights, logits, weights, indices, score, renormalize, s
         _call("ur_route_backward", x, _ptr(grad_weights.contiguous(), torch.float32), x.data_ptr(), stride, code, M,
               x.shape[-1], _ptr(weights, torch.float32), _ptr(indices, torch.int64), indices.shape[-1], score, renormalize,
               scale, grad.data_ptr(), _stream(x))
+    return grad
+
+
+REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = 0, 1, 2  # UR_REDUCE_*
+
+
+def distill_forward(logits, teacher, index, temperature, reduction, need_stats):
+    """logits (..., V), teacher (..., k), index i32 / i64 (..., k) -> loss f32 (rows' shape, or one value), stats"""
+    same_device(logits, teacher, index)
+    code = dtype_code(logits)
+    x, M, stride = rows_of(logits)
+    dev, V = x.device, x.shape[-1]
+    per_row = reduction == REDUCE_NONE
+    loss = torch.empty(logits.shape[:-1] if per_row else (), dtype=torch.float32, device=dev)
+    stats = torch.empty(2 * M + 1, dtype=torch.float32, device=dev) if need_stats else None
+    if not M:
+        return (loss if per_row else loss.zero_()), stats
+    n = _sized("ur_distill_workspace_bytes", M, V, code, reduction)
+    ws = _ws(n, dev)
+    _call("ur_distill_forward", x, x.data_ptr(), stride, code, M, V, _ptr(teacher), dtype_code(teacher), _ptr(index),
+          index.element_size(), index.shape[-1], temperature, reduction, loss.data_ptr(), _ptr(stats, None, True),
+          ws.data_ptr() if n else None, n, _stream(x))
+    return loss, stats
+
+
+def distill_backward(grad_loss, logits, teacher, index, temperature, reduction, stats):
+    """-> grad of logits (their shape and type)"""
+    code = dtype_code(logits)
+    x, M, stride = rows_of(logits)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=x.device)
+    if M:
+        g = grad_loss
+        if reduction == REDUCE_NONE and g.dim() != 1:
+            g = g.reshape(-1)
+        gstride = g.stride(0) if g.dim() else 0
+        if gstride < 0:
+            g, gstride = g.contiguous(), 1
+        _call("ur_distill_backward", x, g.data_ptr(), gstride, x.data_ptr(), stride, code, M, x.shape[-1], _ptr(teacher),
+              dtype_code(teacher), _ptr(index), index.element_size(), index.shape[-1], temperature, reduction,
+              stats.data_ptr(), grad.data_ptr(), _stream(x))
     return grad
