@@ -14,7 +14,9 @@ from torch.nn import functional as F
 
 from . import lighting, native, ops
 from .cameras import FoVPerspectiveCameras, PerspectiveCameras, look_at_view_transform
-from .structures import Meshes, TexturesUV, TexturesVertex  # noqa: F401  (re-exported for callers)
+from .candidates import CandidateImages, chosen_poses
+from .routing import route_candidates
+from .structures import Meshes, TexturesUV, TexturesVertex, repeat  # noqa: F401  (re-exported for callers)
 
 LAYERED_SHADER = True
 SHADING_TYPE = 'raw'
@@ -447,6 +449,23 @@ class Renderer(nn.Module):
         """-> (N, 4, H, W) RGBA"""
         pipeline = self.viz_renderer if viz_purpose else self.renderer
         return pipeline(meshes, R=R, T=T)
+
+    def render_candidates(self, meshes, R, T, scores, top_k, bias=None, viz_purpose=False, **routing):
+        """Renders the `top_k` best of every mesh's K candidate poses R (B,K,3,3), T (B,K,3) under scores (B,K) -- where
+        the reference renders all K (unicorn.py:232-233,295-304).  `bias` and the keyword arguments go to
+        `route_candidates`.  -> CandidateImages(images (B,top_k,4,H,W), routing); a slot without an eligible candidate
+        (index -1, weight 0) shows candidate 0."""
+        B = len(meshes)
+        if scores.dim() != 2 or R.shape != scores.shape + (3, 3) or T.shape != scores.shape + (3,) or len(scores) != B:
+            raise ValueError(f"render_candidates needs R (B,K,3,3), T (B,K,3) and scores (B,K) with B = {B} meshes, got "
+                             f"{tuple(R.shape)}, {tuple(T.shape)}, {tuple(scores.shape)}")
+        choice = route_candidates(scores, top_k, bias=bias, **routing)
+        if B == 0:
+            H, W = (self.viz_renderer if viz_purpose else self.renderer).rasterizer.raster_settings.image_size
+            H, W = (H // 2, W // 2) if viz_purpose else (H, W)
+            return CandidateImages(torch.zeros(0, top_k, 4, H, W, device=R.device), choice)
+        images = self(repeat(meshes, top_k), *chosen_poses(R, T, choice), viz_purpose=viz_purpose)
+        return CandidateImages(images.unflatten(0, (top_k, B)).transpose(0, 1), choice)
 
     def to(self, device):
         super().to(device)
