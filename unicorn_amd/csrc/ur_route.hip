@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kMaxCands = 1024, kMaxTop = 64, kMaxGroups = 64;
 constexpr int kThreads = 256, kWaves = kThreads / 64;
+typedef float f32x4_lds __attribute__((ext_vector_type(4)));
 constexpr int kMaxBlocks = 1024;  // workgroups of the forward = rows of partial counts
 
 struct RouteParams {
@@ -46,6 +47,14 @@ __device__ __forceinline__ uint64_t order_key(double v) {
 __device__ __forceinline__ double key_value(uint64_t k) {
   return __longlong_as_double((long long)((k >> 63) ? (k & 0x7fffffffffffffffull) : ~k));  // (NaN -> NaN)
 }
+__device__ __forceinline__ uint32_t order_key(float v) {
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  const uint32_t k = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+  return v != v ? ~0u : k;
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k);
+}
 
 __device__ __forceinline__ double wave_sum(double v) {
   for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
@@ -53,13 +62,12 @@ __device__ __forceinline__ double wave_sum(double v) {
 }
 
 // ---- the choice in 64 bits, one wave for a row; lane j < k returns slot j's candidate or -1 --------------------------
-// `vals`: LDS of this wave, one double per candidate; `poisoned`: the row's softmax is NaN (a NaN or +inf among its logits).
+// `store`: LDS of this wave, 8 bytes a candidate: first the groups' values, then the keys.
 template <typename T>
-__device__ int choose_wide(const RouteParams& P, const T* __restrict__ row, double* vals, bool& poisoned) {
-  constexpr int kItems = kMaxCands / 64;
+__device__ int choose_wide(const RouteParams& P, const T* __restrict__ row, uint64_t* store) {
   const int lane = threadIdx.x & 63, E = P.cands;
   const double inf = __builtin_inf();
-  double m = -inf, z = 1.0;
+  double m = 0.0, z = 1.0;
   if (!P.sigmoid) {
     float mf = -__builtin_inff();
     for (int e = lane; e < E; e += 64) mf = __builtin_fmaxf(mf, (float)row[e]);
@@ -69,30 +77,27 @@ __device__ int choose_wide(const RouteParams& P, const T* __restrict__ row, doub
     for (int e = lane; e < E; e += 64) z += exp((double)(float)row[e] - m);
     z = wave_sum(z);
   }
-  poisoned = z != z;
-  uint64_t key[kItems];
-#pragma unroll
-  for (int i = 0; i < kItems; ++i) {
-    const int e = lane + 64 * i;
-    key[i] = 0;
-    if (e < E) {
-      const double l = (double)(float)row[e];
-      const double s = P.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - m) / z;
-      const double c = P.bias ? s + (double)P.bias[e] : l;
-      const bool ok = l != -inf && !(P.bias && c == -inf);
-      key[i] = ok ? order_key(c) : 0;
-      // a group's value: by scores where they are added, by the order of the keys else
-      if (P.groups > 1) vals[e] = !ok ? -inf : (P.bias || !P.top2) ? c : s;
-    }
-  }
+  // c of a candidate (by_score: s where c would be the bare logit), -inf where it is not eligible
+  const auto value = [&](int e, bool by_score) {
+    const double l = (double)(float)row[e];
+    if (l == -inf) return -inf;
+    if (!P.bias && !by_score) return l;
+    const double s = P.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - m) / z;
+    return P.bias ? s + (double)P.bias[e] : s;
+  };
+  wave_lds_handoff();
+  uint64_t kept = ~0ull;
   if (P.groups > 1) {
+    for (int e = lane; e < E; e += 64) {
+      const double v = value(e, P.top2);
+      store[e] = v == -inf ? 0 : order_key(v);
+    }
     wave_lds_handoff();
     uint64_t g = 0;
     if (lane < P.groups) {
       uint64_t a = 0, b = 0;  // the two largest (0: none)
       for (int i = 0; i < P.per_group; ++i) {
-        const double v = vals[lane * P.per_group + i];
-        const uint64_t k = v == -inf ? 0 : order_key(v);
+        const uint64_t k = store[lane * P.per_group + i];
         b = k > a ? a : (k > b ? k : b);
         a = k > a ? k : a;
       }
@@ -103,21 +108,22 @@ __device__ int choose_wide(const RouteParams& P, const T* __restrict__ row, doub
       const uint64_t other = __shfl(g, o);
       rank += other > g || (other == g && o < lane);
     }
-    const uint64_t kept = __ballot(lane < P.groups && rank < P.top_groups);
-#pragma unroll
-    for (int i = 0; i < kItems; ++i)
-      if (lane + 64 * i < E && !((kept >> ((lane + 64 * i) / P.per_group)) & 1)) key[i] = 0;
-    wave_lds_handoff();  // (the next row writes `vals` again)
+    kept = __ballot(lane < P.groups && rank < P.top_groups);
+    wave_lds_handoff();
   }
+  for (int e = lane; e < E; e += 64) {
+    const double v = value(e, false);
+    store[e] = (v == -inf || (P.groups > 1 && !((kept >> (e / P.per_group)) & 1))) ? 0 : order_key(v);
+  }
+  wave_lds_handoff();
   int mine = -1;
   for (int r = 0; r < P.top_k; ++r) {
     uint64_t best = 0;
     int at = E;
-#pragma unroll
-    for (int i = 0; i < kItems; ++i)
-      if (key[i] > best) {
-        best = key[i];
-        at = lane + 64 * i;
+    for (int e = lane; e < E; e += 64)
+      if (store[e] > best) {
+        best = store[e];
+        at = e;
       }
     for (int o = 32; o; o >>= 1) {
       const uint64_t ob = __shfl_xor(best, o);
@@ -129,10 +135,9 @@ __device__ int choose_wide(const RouteParams& P, const T* __restrict__ row, doub
     }
     if (best == 0) break;
     if (lane == r) mine = at;
-#pragma unroll
-    for (int i = 0; i < kItems; ++i)
-      if (lane + 64 * i == at) key[i] = 0;
+    if ((at & 63) == lane) store[at] = 0;  // (read by this lane only)
   }
+  wave_lds_handoff();
   return mine;
 }
 
@@ -177,29 +182,308 @@ __device__ __forceinline__ void row_softmax(const T* __restrict__ row, int E, in
   if (z == 0.0f) z = 1.0f;  // nothing eligible: every score is 0
 }
 
-template <typename T>
+// ---- forward: LPR lanes a row, IPL consecutive candidates a lane -----------------------------------------------------
+// The choice is made in fp32 and redone in 64 bits (choose_wide) for the rows where fp32 cannot tell: with a bias, when two
+// neighbours of the order -- or the last group taken and the first one left -- are closer than fp32's error and are not the
+// same (logit, bias) twice.  Without a bias the logits themselves are compared and nothing has to be redone.
+//
+// The top-k is not taken by k rounds of a maximum: the (k+1)-th largest of the lanes' maxima is a lower bound of the (k+1)-th
+// largest candidate; the few candidates that reach it (about 10 of 256) go to a list in LDS as (key, index) and each finds its rank
+// by counting the larger ones.
+
+template <int L>
+__device__ __forceinline__ uint32_t max_lanes(uint32_t v) {
+  const auto mx = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+  if constexpr (L >= 2) v = mx(v, dpp32<kDppXor1>(v));
+  if constexpr (L >= 4) v = mx(v, dpp32<kDppXor2>(v));
+  if constexpr (L >= 8) v = mx(v, dpp32<kDppHalfMirror>(v));
+  if constexpr (L >= 16) v = mx(v, dpp32<kDppMirror>(v));
+  if constexpr (L >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = mx(r[0], r[1]);
+  }
+  if constexpr (L >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = mx(r[0], r[1]);
+  }
+  return v;
+}
+
+// how many of the values that a row's other 15 lanes hold (two a lane) are >= v, >= w
+template <int kRor>
+__device__ __forceinline__ void count_ge16(uint32_t v, uint32_t w, int& nv, int& nw) {
+  if constexpr (kRor > 0) {
+    const uint32_t a = dpp32<0x120 + kRor>(v), b = dpp32<0x120 + kRor>(w);
+    nv += (a >= v) + (b >= v);
+    nw += (a >= w) + (b >= w);
+    count_ge16<kRor - 1>(v, w, nv, nw);
+  }
+}
+
+// A lower bound (at least 1) of the (k+1)-th largest key, from the maxima of two sets of keys a lane.  (Two, because groups
+// that were not taken leave lanes empty: with half of 16 lanes left, their 16 sets still bound the 9th largest.)
+template <int LPR>
+__device__ __forceinline__ uint32_t prune_bound(uint32_t v, uint32_t w, int k) {
+  uint32_t bound;
+  if (LPR >= 16 && k + 1 <= 32) {  // 32 sets: lanes 16, 32, 48 apart are put together
+    if constexpr (LPR >= 32) {
+      const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false), q = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+      v = max(r[0], r[1]);
+      w = max(q[0], q[1]);
+    }
+    if constexpr (LPR >= 64) {
+      const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false), q = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+      v = max(r[0], r[1]);
+      w = max(q[0], q[1]);
+    }
+    int nv = 1 + (w >= v), nw = 1 + (v >= w);
+    count_ge16<15>(v, w, nv, nw);
+    bound = max_lanes<16>(max(nv >= k + 1 ? v : 0u, nw >= k + 1 ? w : 0u));
+  } else {
+    int nv = 0, nw = 0;
+    for (int i = 0; i < LPR; ++i) {
+      const uint32_t a = (uint32_t)__shfl((int)v, i, LPR), b = (uint32_t)__shfl((int)w, i, LPR);
+      nv += (a >= v) + (b >= v);
+      nw += (a >= w) + (b >= w);
+    }
+    bound = max_lanes<LPR>(max(nv >= k + 1 ? v : 0u, nw >= k + 1 ? w : 0u));
+  }
+  return bound > 1u ? bound : 1u;
+}
+
+// sum of the lanes before this one, inside groups of LPR lanes
+template <int LPR>
+__device__ __forceinline__ int lanes_before(int v, int t) {
+  int incl = v;
+#pragma unroll
+  for (int o = 1; o < LPR; o <<= 1) {
+    const int up = __shfl_up(incl, o, LPR);
+    if (t >= o) incl += up;
+  }
+  return incl - v;
+}
+
+// the hardware's exponential (1 ulp) of the argument rounded to base 2
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
+
+template <typename T, int IPL>
+__device__ __forceinline__ void load_items(const T* __restrict__ row, int first, int E, float (&l)[IPL]) {
+  struct __attribute__((packed, aligned(sizeof(T)))) Items { T v[IPL]; };
+  if (first + IPL <= E) {
+    const Items it = *reinterpret_cast<const Items*>(row + first);
+#pragma unroll
+    for (int i = 0; i < IPL; ++i) l[i] = (float)it.v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < IPL; ++i) l[i] = first + i < E ? (float)row[first + i] : -__builtin_inff();
+  }
+}
+
+template <typename T, int LPR, int IPL>
 __global__ void __launch_bounds__(kThreads) k_route_fwd(const RouteParams P) {
-  __shared__ int hist[kMaxCands];
-  __shared__ double vals[kWaves][kMaxCands];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int e = threadIdx.x; e < P.cands; e += kThreads) hist[e] = 0;
+  constexpr int R = 64 / LPR, kRow = LPR * IPL;
+  constexpr float kInf = __builtin_inff();
+  __shared__ int hist[kRow];
+  __shared__ uint64_t lists[kWaves][R * kRow];
+  __shared__ uint64_t slot_store[kWaves][R * (LPR + 1)];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / LPR, t = lane % LPR;
+  uint64_t* list = lists[wave] + sub * kRow;
+  uint64_t* slots = slot_store[wave] + sub * (LPR + 1);
+  float* vals = reinterpret_cast<float*>(lists[wave]) + sub * kRow;
+  const int E = P.cands, first = t * IPL, k = P.top_k, G = P.groups, per = P.per_group;
+  for (int e = threadIdx.x; e < E; e += kThreads) hist[e] = 0;
   __syncthreads();
-  for (int64_t row = (int64_t)blockIdx.x * kWaves + wave; row < P.rows; row += (int64_t)gridDim.x * kWaves) {
-    const T* l = static_cast<const T*>(P.logits) + row * P.stride;
-    bool poisoned;
-    const int at = choose_wide<T>(P, l, vals[wave], poisoned);
-    float m = 0.0f, z = 1.0f;
-    if (!P.sigmoid && !P.renormalize) row_softmax<T, 64>(l, P.cands, lane, m, z);
-    const Chosen c = chosen_share<64>(P.sigmoid, P.renormalize, at >= 0 ? (float)l[at] : 0.0f, at >= 0, m, z);
-    if (lane < P.top_k) {
-      P.weights[row * P.top_k + lane] = poisoned ? __builtin_nanf("") : P.scale * c.share;
-      P.indices[row * P.top_k + lane] = at;
+  const bool group_scores = G > 1 && P.top2 && !P.bias;  // groups are compared by sums of scores, candidates by logits
+  const bool need_scores = P.bias != nullptr || group_scores;
+  const bool need_softmax = !P.sigmoid && (need_scores || !P.renormalize);
+  // whole groups of lanes per group of candidates, a power of two of them: groups are formed in registers
+  const int lanes_per = per / IPL;
+  const bool whole = per % IPL == 0 && (lanes_per & (lanes_per - 1)) == 0;
+  int share = LPR;  // else: lanes that scan one group in LDS
+  while (share > 1 && LPR / share < G) share >>= 1;
+  float bias[IPL];
+#pragma unroll
+  for (int i = 0; i < IPL; ++i) bias[i] = (P.bias && first + i < E) ? P.bias[first + i] : 0.0f;
+
+  const int64_t row_groups = (P.rows + kWaves * R - 1) / (kWaves * R);
+  for (int64_t rg = blockIdx.x; rg < row_groups; rg += gridDim.x) {
+    const int64_t want = (rg * kWaves + wave) * R + sub;
+    const bool mine = want < P.rows;
+    const int64_t row = mine ? want : P.rows - 1;
+    const T* src = static_cast<const T*>(P.logits) + row * P.stride;
+    float l[IPL];
+    load_items<T, IPL>(src, first, E, l);
+
+    // err: bound of two scores' errors.  sigmoid: s (1 - s) (|l| 2^-23.4 + 2^-23) of the exponential, 2^-23 of the
+    // reciprocal, 2^-24 of the sum: below 2^-22 each.  softmax, relative to its largest score 1 / z: as much of the
+    // exponential and up to 30 roundings of z, below 2^-19 each.
+    float m = 0.0f, z = 1.0f, inv_z = 1.0f, err = 0x1p-20f;
+    if (need_softmax) {
+      float mf = l[0];
+#pragma unroll
+      for (int i = 1; i < IPL; ++i) mf = __builtin_fmaxf(mf, l[i]);
+      mf = reduce_lanes<LPR, OpMax>(mf);
+      m = mf == -kInf ? 0.0f : mf;
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < IPL; ++i) sum += fast_exp(l[i] - m);
+      z = reduce_lanes<LPR, OpSum>(sum);
+      if (z == 0.0f) z = 1.0f;
+      inv_z = 1.0f / z;
+      err = 0x1p-17f * inv_z;
+    }
+    uint32_t key[IPL], gkey[IPL];
+#pragma unroll
+    for (int i = 0; i < IPL; ++i) {
+      float c = l[i], s = l[i];
+      if (need_scores) {
+        s = P.sigmoid ? __builtin_amdgcn_rcpf(1.0f + fast_exp(-l[i])) : fast_exp(l[i] - m) * inv_z;
+        if (P.bias) c = s + bias[i];
+      }
+      const bool ok = l[i] != -kInf && c != -kInf;
+      key[i] = ok ? order_key(c) : 0u;
+      gkey[i] = group_scores ? (ok ? order_key(s) : 0u) : key[i];
+    }
+
+    bool close = false;  // fp32 cannot tell
+    if (G > 1) {
+      uint32_t a = 0, b = 0;  // the two largest of this lane's group (0: none)
+      int width;              // lanes that hold the same group
+      if (whole) {
+        width = lanes_per;
+#pragma unroll
+        for (int i = 0; i < IPL; ++i) {
+          const uint32_t lo = min(a, gkey[i]);
+          a = max(a, gkey[i]);
+          b = max(b, lo);
+        }
+      } else {
+        width = share;
+        wave_lds_handoff();
+#pragma unroll
+        for (int i = 0; i < IPL; ++i) vals[first + i] = __uint_as_float(gkey[i]);
+        wave_lds_handoff();
+        const int g = t / share;
+        if (g < G)
+          for (int i = t % share; i < per; i += share) {
+            const uint32_t v = __float_as_uint(vals[g * per + i]);
+            const uint32_t lo = min(a, v);
+            a = max(a, v);
+            b = max(b, lo);
+          }
+        wave_lds_handoff();
+      }
+      for (int o = 1; o < width; o <<= 1) {
+        const uint32_t a2 = (uint32_t)__shfl_xor((int)a, o), b2 = (uint32_t)__shfl_xor((int)b, o);
+        b = max(min(a, a2), max(b, b2));
+        a = max(a, a2);
+      }
+      const uint32_t g = (P.top2 && a && b) ? order_key(key_value(a) + key_value(b)) : a;
+      const int my_group = t / width;
+      int rank = 0;
+      uint32_t above = ~0u;  // the smallest of the groups that come before this one
+      for (int o = 0; o < G; ++o) {
+        const uint32_t other = (uint32_t)__shfl((int)g, o * width, LPR);
+        const bool before = other > g || (other == g && o < my_group);
+        rank += before;
+        if (before) above = min(above, other);
+      }
+      const bool taken = my_group < G && rank < P.top_groups;
+      if (need_scores && my_group < G && rank == P.top_groups && g != 0) {
+        const float va = key_value(above), vg = key_value(g);
+        close = va - vg <= 2.0f * err + 0x1p-21f * (fabsf(va) + fabsf(vg));
+      }
+      const uint64_t kept = (__ballot(taken) >> (sub * LPR));  // bit t: lane t's group is taken
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < IPL; ++i) key[i] = taken ? key[i] : 0u;
+      } else {
+        int at = first / per, in = first % per;
+#pragma unroll
+        for (int i = 0; i < IPL; ++i) {
+          if (at >= G || !((kept >> (at * share)) & 1)) key[i] = 0u;
+          if (++in == per) {
+            in = 0;
+            ++at;
+          }
+        }
+      }
+    }
+
+    // the candidates that can be among the k + 1 largest
+    uint32_t bound = 1u;
+    if constexpr (IPL > 1) {
+      uint32_t v = key[0], w = key[IPL / 2];
+#pragma unroll
+      for (int i = 1; i < IPL / 2; ++i) {
+        v = max(v, key[i]);
+        w = max(w, key[IPL / 2 + i]);
+      }
+      bound = prune_bound<LPR>(v, w, k);
+    }
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < IPL; ++i) count += key[i] >= bound;
+    const int before = lanes_before<LPR>(count, t);
+    const int n = __shfl(before + count, LPR - 1, LPR);
+    wave_lds_handoff();
+    list[t] = 0;  // (the first LPR entries are all read below)
+    int pos = before;
+#pragma unroll
+    for (int i = 0; i < IPL; ++i)
+      if (key[i] >= bound) list[pos++] = ((uint64_t)key[i] << 32) | (uint32_t)(kMaxCands - (first + i));
+    for (int j = t; j <= k; j += LPR) slots[j] = 0;
+    wave_lds_handoff();
+    int n_max = n;
+    if constexpr (R > 1) n_max = (int)reduce_lanes<64, OpMax>((float)n);
+    if (n_max <= LPR) {
+      const uint64_t own = list[t];
+      int rank = 0;
+#pragma unroll 4
+      for (int i = 0; i < n_max; ++i) rank += list[i] > own;
+      if (own && rank <= k) slots[rank] = own;
+    } else {
+      for (int j0 = 0; j0 < n_max; j0 += LPR) {
+        const int j = j0 + t;
+        const uint64_t own = j < n ? list[j] : ~0ull;
+        int rank = 0;
+        for (int i = 0; i < n_max; ++i) rank += i < n && list[i] > own;
+        if (j < n && rank <= k) slots[rank] = own;
+      }
+    }
+    wave_lds_handoff();
+
+    const uint64_t got = t < k ? slots[t] : 0;
+    int at = got ? kMaxCands - (int)(uint32_t)got : -1;
+    if (P.bias && got) {
+      const uint64_t next = slots[t + 1];
+      const float c = key_value((uint32_t)(got >> 32)), c2 = key_value((uint32_t)(next >> 32));
+      if (next && c - c2 <= err + 0x1p-22f * (fabsf(c) + fabsf(c2))) {
+        const int at2 = kMaxCands - (int)(uint32_t)next;
+        close |= !((float)src[at] == (float)src[at2] && P.bias[at] == P.bias[at2]);
+      }
+    }
+    uint64_t redo = __ballot(close && mine);
+    while (redo) {  // (the whole wave, one row at a time)
+      const int r = __builtin_ctzll(redo) / LPR;
+      const int64_t wide_row = (rg * kWaves + wave) * R + r;
+      const int chosen = choose_wide<T>(P, static_cast<const T*>(P.logits) + wide_row * P.stride, lists[wave]);
+      if (lane < k) slot_store[wave][r * (LPR + 1) + lane] = chosen < 0 ? 0 : (uint64_t)(kMaxCands - chosen);
+      wave_lds_handoff();
+      if (sub == r && t < k) at = slots[t] ? kMaxCands - (int)(uint32_t)slots[t] : -1;
+      redo &= R == 1 ? 0ull : ~(((1ull << (LPR & 63)) - 1) << (r * LPR));
+    }
+
+    const Chosen ch = chosen_share<LPR>(P.sigmoid, P.renormalize, at >= 0 ? (float)src[at] : 0.0f, at >= 0, m, z);
+    if (mine && t < k) {
+      P.weights[row * k + t] = z != z ? z : P.scale * ch.share;  // (a NaN in a softmax is in every score)
+      P.indices[row * k + t] = at;
       if (at >= 0) atomicAdd(&hist[at], 1);
     }
   }
   __syncthreads();
-  int32_t* out = P.parts > 1 ? P.ws + (int64_t)blockIdx.x * P.cands : P.counts;
-  for (int e = threadIdx.x; e < P.cands; e += kThreads) out[e] = hist[e];
+  int32_t* out = P.parts > 1 ? P.ws + (int64_t)blockIdx.x * E : P.counts;
+  for (int e = threadIdx.x; e < E; e += kThreads) out[e] = hist[e];
 }
 
 // counts = the sums of the workgroups' counts: 32 candidates a workgroup, 32 groups of threads over the partial rows
@@ -222,46 +506,57 @@ __global__ void __launch_bounds__(1024) k_route_counts(const RouteParams P) {
 //     and nothing cancels where one choice has nearly all the weight;
 //     softmax: dl_j = scale share_j d_j for the chosen, exactly 0 for all others; sigmoid: times (1 - s_j)
 //   not renormalised: sigmoid: dl_j = scale dw_j s_j (1 - s_j); softmax: dl_e = s_e (ds_e - sum_j ds_j s_j), every candidate
-template <typename T>
+// A row of gradients is put together in LDS (zeros and the k chosen) and stored in 16-byte pieces.
+template <typename T, int LPR>
 __global__ void __launch_bounds__(kThreads) k_route_bwd(const RouteParams P) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
-  if (row >= P.rows) return;  // (whole waves)
+  constexpr int R = 64 / LPR, kRow = LPR * 16, N = Elem<T>::kN;
+  __shared__ __align__(16) float rows[kWaves][R * kRow];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / LPR, t = lane % LPR;
+  float* acc = rows[wave] + sub * kRow;
+  const int64_t want = ((int64_t)blockIdx.x * kWaves + wave) * R + sub;
+  const bool mine = want < P.rows;
+  const int64_t row = mine ? want : P.rows - 1;
   const T* l = static_cast<const T*>(P.logits) + row * P.stride;
-  T* out = static_cast<T*>(P.grad) + row * P.cands;
-  const int64_t slot = lane < P.top_k ? P.indices[row * P.top_k + lane] : -1;
+  const int64_t slot = t < P.top_k ? P.indices[row * P.top_k + t] : -1;
   const bool filled = slot >= 0 && slot < P.cands;
   const int at = filled ? (int)slot : -1;
-  const float dw = filled ? P.grad_w[row * P.top_k + lane] : 0.0f;
+  const float dw = filled ? P.grad_w[row * P.top_k + t] : 0.0f;
   const bool dense = !P.sigmoid && !P.renormalize;
+  // a NaN in a softmax is in every score: the forward left it in every weight of the row
+  const float first = P.weights[row * P.top_k];
+  const float base = !P.sigmoid && first != first ? first : 0.0f;
+  for (int e = 4 * t; e < P.cands; e += 4 * LPR) *reinterpret_cast<f32x4_lds*>(acc + e) = f32x4_lds{base, base, base, base};
   float m = 0.0f, z = 1.0f;
-  if (dense) row_softmax<T, 64>(l, P.cands, lane, m, z);
-  const Chosen c = chosen_share<64>(P.sigmoid, P.renormalize, filled ? (float)l[at] : 0.0f, filled, m, z);
+  if (dense) row_softmax<T, LPR>(l, P.cands, t, m, z);
+  const Chosen c = chosen_share<LPR>(P.sigmoid, P.renormalize, filled ? (float)l[at] : 0.0f, filled, m, z);
   float g;
   if (P.renormalize) {
     float d = 0.0f;
     for (int i = 0; i < P.top_k; ++i) {
-      const float wi = __shfl(c.share, i), di = __shfl(dw, i);
+      const float wi = __shfl(c.share, i, LPR), di = __shfl(dw, i, LPR);
       d = __builtin_fmaf(wi, dw - di, d);
     }
     g = P.scale * c.share * d * c.comp;
   } else {
-    g = P.scale * dw * c.share * c.comp;  // (softmax: ds_j s_j)
+    g = P.scale * dw * (dense ? 1.0f : c.share * c.comp);
   }
-  const float dot = dense ? reduce_lanes<64, OpSum>(filled ? g : 0.0f) : 0.0f;
-  // a NaN in a softmax is in every score: the forward left it in every weight of the row
-  const float first = P.weights[row * P.top_k];
-  const bool poisoned = !P.sigmoid && first != first;
-  for (int base = 0; base < P.cands; base += 64) {  // (whole waves: lanes read each other's slots)
-    const int e = base + lane;
-    float v = poisoned ? first : 0.0f;
-    if (dense && e < P.cands) v = -(expf((float)l[e] - m) / z) * dot;
-    for (int j = 0; j < P.top_k; ++j) {
-      const int aj = __shfl(at, j);
-      const float gj = __shfl(g, j);
-      if (aj == e) v += gj;
+  const float dot = dense ? reduce_lanes<LPR, OpSum>(filled ? g * c.share : 0.0f) : 0.0f;
+  wave_lds_handoff();
+  if (filled) acc[at] = base + g;
+  wave_lds_handoff();
+  if (!mine) return;
+  T* out = static_cast<T*>(P.grad) + row * P.cands;
+  for (int e = t * N; e < P.cands; e += LPR * N) {
+    typename Elem<T>::Vec o;
+    if (dense) {
+      const auto v = load16<T>(l, e, P.cands, (T)-__builtin_inff());
+#pragma unroll
+      for (int j = 0; j < N; ++j) o[j] = (T)(expf((float)v[j] - m) / z * (acc[e + j] - dot));
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) o[j] = (T)acc[e + j];
     }
-    if (e < P.cands) out[e] = (T)v;
+    store16<T>(out, e, P.cands, o);
   }
 }
 
@@ -278,7 +573,40 @@ int check_common(const void* logits, int64_t stride, int dtype, int64_t rows, in
   return UR_OK;
 }
 
-int route_parts(int64_t rows) { return (int)std::min<int64_t>(ceil_div(rows, kWaves), kMaxBlocks); }
+// Lanes a row and candidates a lane: the fewest lanes that hold the row 16 a lane, one choice and one group a lane (8 lanes:
+// rows of at most 8 candidates) -- lane exchanges cost the same for one row as for eight.  Where a lane holds several
+// candidates there is one lane more than choices, or prune_bound has nothing to go by.
+struct RouteShape { int lpr, ipl; };
+RouteShape route_shape(int cands, int top_k, int groups) {
+  const int need = std::max(top_k, groups);
+  RouteShape s{64, 1};
+  if (cands <= 8) s.lpr = 8;
+  else if (cands <= 256 && need <= (cands <= 16 ? 16 : 15)) s.lpr = 16;
+  else if (cands <= 512 && need <= (cands <= 32 ? 32 : 31)) s.lpr = 32;
+  while (s.lpr * s.ipl < cands) s.ipl *= 2;
+  if (s.lpr > 16) s.ipl = s.ipl == 2 ? 4 : s.ipl == 8 ? 16 : s.ipl;  // (1, 4 and 16 only: these rows are rare)
+  return s;
+}
+
+int route_parts(int64_t rows, int lpr) { return (int)std::min<int64_t>(ceil_div(rows, kWaves * (64 / lpr)), kMaxBlocks); }
+
+template <typename T>
+void launch_fwd(const RouteParams& P, RouteShape s, hipStream_t st) {
+#define UR_ROUTE(L, I) \
+  if (s.lpr == L && s.ipl == I) k_route_fwd<T, L, I><<<P.parts, kThreads, 0, st>>>(P);
+  UR_ROUTE(8, 1) UR_ROUTE(16, 1) UR_ROUTE(16, 2) UR_ROUTE(16, 4) UR_ROUTE(16, 8) UR_ROUTE(16, 16)
+  UR_ROUTE(32, 1) UR_ROUTE(32, 4) UR_ROUTE(32, 16) UR_ROUTE(64, 1) UR_ROUTE(64, 4) UR_ROUTE(64, 16)
+#undef UR_ROUTE
+}
+
+template <typename T>
+void launch_bwd(const RouteParams& P, int lpr, hipStream_t st) {
+  const unsigned grid = (unsigned)ceil_div(P.rows, kWaves * (64 / lpr));
+  if (lpr == 8) k_route_bwd<T, 8><<<grid, kThreads, 0, st>>>(P);
+  else if (lpr == 16) k_route_bwd<T, 16><<<grid, kThreads, 0, st>>>(P);
+  else if (lpr == 32) k_route_bwd<T, 32><<<grid, kThreads, 0, st>>>(P);
+  else k_route_bwd<T, 64><<<grid, kThreads, 0, st>>>(P);
+}
 
 }  // namespace
 
@@ -287,7 +615,7 @@ extern "C" {
 int64_t ur_route_workspace_bytes(int64_t rows, int cands) {
   if (rows <= 0 || cands <= 0 || rows > 0x7fffffff || cands > kMaxCands)
     return set_error(UR_ERR_INVALID_ARG, "bad rows or cands");
-  const int parts = route_parts(rows);
+  const int parts = route_parts(rows, 64);  // (the most any shape needs)
   return parts > 1 ? (int64_t)parts * cands * 4 : 0;
 }
 
@@ -313,11 +641,12 @@ int ur_route_forward(const void* logits, int64_t row_stride, int dtype, const fl
   P.groups = groups; P.per_group = cands / groups; P.top_groups = top_groups;
   P.sigmoid = score == UR_SCORE_SIGMOID; P.top2 = group_score == UR_GROUP_TOP2; P.renormalize = renormalize != 0;
   P.scale = scale; P.weights = weights; P.indices = indices; P.counts = counts;
-  P.ws = static_cast<int32_t*>(workspace); P.parts = route_parts(rows);
+  const RouteShape shape = route_shape(cands, top_k, groups);
+  P.ws = static_cast<int32_t*>(workspace); P.parts = route_parts(rows, shape.lpr);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == UR_F32) k_route_fwd<float><<<P.parts, kThreads, 0, st>>>(P);
-  else if (dtype == UR_F16) k_route_fwd<_Float16><<<P.parts, kThreads, 0, st>>>(P);
-  else k_route_fwd<__bf16><<<P.parts, kThreads, 0, st>>>(P);
+  if (dtype == UR_F32) launch_fwd<float>(P, shape, st);
+  else if (dtype == UR_F16) launch_fwd<_Float16>(P, shape, st);
+  else launch_fwd<__bf16>(P, shape, st);
   if (P.parts > 1) k_route_counts<<<(unsigned)ceil_div(cands, 32), 1024, 0, st>>>(P);
   return launch_status("ur_route_forward");
 }
@@ -334,10 +663,10 @@ int ur_route_backward(const float* grad_weights, const void* logits, int64_t row
   P.sigmoid = score == UR_SCORE_SIGMOID; P.renormalize = renormalize != 0; P.scale = scale;
   P.indices = const_cast<int64_t*>(indices); P.grad_w = grad_weights; P.weights = const_cast<float*>(weights); P.grad = grad_logits;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const unsigned grid = (unsigned)ceil_div(rows, kWaves);
-  if (dtype == UR_F32) k_route_bwd<float><<<grid, kThreads, 0, st>>>(P);
-  else if (dtype == UR_F16) k_route_bwd<_Float16><<<grid, kThreads, 0, st>>>(P);
-  else k_route_bwd<__bf16><<<grid, kThreads, 0, st>>>(P);
+  const int lpr = cands <= 8 ? 8 : cands <= 256 && top_k <= 16 ? 16 : cands <= 512 && top_k <= 32 ? 32 : 64;
+  if (dtype == UR_F32) launch_bwd<float>(P, lpr, st);
+  else if (dtype == UR_F16) launch_bwd<_Float16>(P, lpr, st);
+  else launch_bwd<__bf16>(P, lpr, st);
   return launch_status("ur_route_backward");
 }
 
