@@ -371,11 +371,11 @@ int ur_route_backward(const float* grad_weights, const void* logits, int64_t row
 #define UR_REDUCE_MEAN 2
 int64_t ur_distill_workspace_bytes(int64_t rows, int64_t cols, int dtype, int reduction);
 int ur_distill_forward(const void* logits, int64_t row_stride, int dtype, int64_t rows, int64_t cols, const void* teacher,
-                       int teacher_dtype, const void* index, int index_bytes, int top, float temperature, int reduction,
+                       int teacher_dtype, const void* index, int index_bytes, int top, double temperature, int reduction,
                        float* loss, float* stats, void* workspace, size_t workspace_bytes, void* stream);
 int ur_distill_backward(const float* grad_loss, int64_t grad_stride, const void* logits, int64_t row_stride, int dtype,
                         int64_t rows, int64_t cols, const void* teacher, int teacher_dtype, const void* index,
-                        int index_bytes, int top, float temperature, int reduction, const float* stats,
+                        int index_bytes, int top, double temperature, int reduction, const float* stats,
                         void* grad_logits, void* stream);
 
 #ifdef __cplusplus

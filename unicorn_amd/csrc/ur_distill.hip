@@ -5,8 +5,8 @@
 //   loss = T^2 sum_j p_j (log p_j - log q_{i_j})          dz_v = g T (q_v - sum_{j: i_j = v} p_j)
 //
 // Bound by memory: the forward reads z once (running maximum and sum of exponentials), the backward reads it again and
-// writes the gradient.  Sums are fp32; the k-slot arithmetic, a difference of logarithms that is small where the student has
-// learnt, is in 64 bits.
+// writes the gradient.  Sums are fp32; log p - log q, a difference that is small where the student has learnt, is formed in 64
+// bits.
 #include "ur_rows.h"
 
 #include <algorithm>
@@ -15,9 +15,10 @@ using namespace ur;
 
 namespace {
 
-constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kMaxTop = 1024;  // slots of a row: the backward keeps their classes and shares in LDS
+constexpr double kLog2e = 1.44269504088896340736;
+constexpr int kThreads = 256;   // workgroups that take several rows
+constexpr int kMaxTop = 1024;   // slots of a row: the backward keeps their classes and shares in LDS
+constexpr int kGroupTop = 64;   // ... where a workgroup takes several rows
 
 struct DistillParams {
   const void* z;
@@ -28,13 +29,15 @@ struct DistillParams {
   const void* index;
   bool index64;
   int top;
-  float temperature, inv_t;
+  double temperature;
+  float scale;     // log2(e) / T
+  double scale64;  // the same in 64 bits
   float* stats;  // (rows, 2): maximum of z, sum of exp((z - max) / T)
   float* loss;   // (rows) or one value
   int reduction;
-  float* row_loss;  // rows that are reduced: their losses ...
-  float* taught;    // ... and 1 where the row has a teacher; backward: factor of the reduction (one value)
-  float* ws;        // long rows: (rows, splits, 2) partial maxima and sums
+  double* partial;  // reductions: (partials, 2) sums of losses and numbers of rows that have a teacher
+  int64_t partials;
+  float* split_stats;  // split rows: (rows, splits, 2) maxima and sums of the parts
   int splits;
   int64_t chunk;
   const float* g;
@@ -47,8 +50,17 @@ __device__ __forceinline__ int64_t slot_class(const DistillParams& P, int64_t ro
   return P.index64 ? static_cast<const int64_t*>(P.index)[i] : (int64_t)static_cast<const int32_t*>(P.index)[i];
 }
 
-// exp((v - m) / T); an infinite maximum would make inf - inf of the equal ones, as the definition does
-__device__ __forceinline__ float exp_diff(float v, float m, float scale) { return exp2f((v - m) * scale); }
+// exp((v - m) / T), scale = log2(e) / T, by the hardware's exponential (1 ulp); an infinite maximum makes inf - inf of the
+// equal ones, as the definition does
+__device__ __forceinline__ float exp_diff(float v, float m, float scale) { return __builtin_amdgcn_exp2f((v - m) * scale); }
+
+// exp((v - m) / T) to 2 ulp whatever the size of the argument: the argument is formed in 64 bits and split into a whole
+// power of two and a rest in [-1/2, 1/2] (a slot's share of the teacher; a 64-bit exponential costs ten times as much)
+__device__ __forceinline__ float exp_slot(float v, float m, double scale) {
+  const double y = ((double)v - (double)m) * scale, whole = rint(y);
+  if (y < -150.0) return 0.0f;
+  return __builtin_ldexpf(__builtin_amdgcn_exp2f((float)(y - whole)), (int)whole);
+}
 
 // merges (m, s) of two sets of numbers: s is relative to m; m = -inf with s = 0 is the empty set
 __device__ __forceinline__ void merge(float& m, float& s, float m2, float s2, float scale) {
@@ -61,25 +73,48 @@ __device__ __forceinline__ void merge(float& m, float& s, float m2, float s2, fl
   m = top;
 }
 
-// running maximum and sum of row elements [c0, c1), threads t, t + n, ... of a group
-template <typename T>
+// Running maximum and sum of row elements [c0, c1), threads t, t + n, ... of a group: B loads at a time, one rescaling of the
+// sum for each batch that holds a new maximum.
+template <typename T, int B>
+__device__ __forceinline__ void add_batch(const typename Elem<T>::Vec (&v)[B], float scale, float& m, float& s) {
+  constexpr int N = Elem<T>::kN;
+  float top = (float)v[0][0];
+#pragma unroll
+  for (int b = 0; b < B; ++b)
+#pragma unroll
+    for (int j = 0; j < N; ++j) top = __builtin_fmaxf(top, (float)v[b][j]);
+  if (top > m) {
+    s = m == -__builtin_inff() ? s : s * exp_diff(m, top, scale);
+    m = top;
+  }
+  const float ref = m == -__builtin_inff() ? 0.0f : m;  // (nothing but -inf so far: every term is 0)
+  float part[B] = {};
+#pragma unroll
+  for (int b = 0; b < B; ++b)
+#pragma unroll
+    for (int j = 0; j < N; ++j) part[b] += exp_diff((float)v[b][j], ref, scale);
+#pragma unroll
+  for (int b = 0; b < B; ++b) s += part[b];
+}
+
+template <typename T, int B>
 __device__ __forceinline__ void row_part(const T* __restrict__ z, int64_t c0, int64_t c1, int t, int n, float scale, float& m,
                                          float& s) {
   constexpr int N = Elem<T>::kN;
+  using Vec = typename Elem<T>::Vec;
   m = -__builtin_inff();
   s = 0.0f;
-  for (int64_t col = c0 + (int64_t)t * N; col < c1; col += (int64_t)n * N) {
-    const auto v = load16<T>(z, col, c1, (T)-__builtin_inff());
-    float top = (float)v[0];
+  const int64_t step = (int64_t)n * N;
+  for (int64_t col = c0 + (int64_t)t * N; col < c1; col += B * step) {
+    Vec v[B];
+    if (col + (B - 1) * step + N <= c1) {
 #pragma unroll
-    for (int j = 1; j < N; ++j) top = __builtin_fmaxf(top, (float)v[j]);
-    if (top > m) {
-      s = m == -__builtin_inff() ? s : s * exp_diff(m, top, scale);
-      m = top;
+      for (int b = 0; b < B; ++b) v[b] = *reinterpret_cast<const Vec*>(z + col + b * step);
+    } else {
+#pragma unroll
+      for (int b = 0; b < B; ++b) v[b] = load16<T>(z, col + b * step, c1, (T)-__builtin_inff());
     }
-    const float ref = m == -__builtin_inff() ? 0.0f : m;  // (nothing but -inf so far: every term is 0)
-#pragma unroll
-    for (int j = 0; j < N; ++j) s += exp_diff((float)v[j], ref, scale);
+    add_batch<T, B>(v, scale, m, s);
   }
 }
 
@@ -91,114 +126,188 @@ __device__ __forceinline__ void merge_lanes(float& m, float& s, float scale) {
   m = top;
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+template <int L>
+__device__ __forceinline__ double sum_lanes(double v) {
+  for (int o = L / 2; o; o >>= 1) v += __shfl_xor(v, o);
   return v;
 }
-__device__ __forceinline__ double wave_max(double v) {
-  for (int o = 32; o; o >>= 1) v = fmax(v, __shfl_xor(v, o));
-  return v;
+template <int L>
+__device__ __forceinline__ bool any_lane(bool v) {
+  const uint64_t b = __ballot(v);
+  if (L == 64) return b != 0;
+  return ((b >> ((threadIdx.x & 63) / L * L)) & ((1ull << (L & 63)) - 1)) != 0;
 }
 
-// The teacher of a row, by one wave: maximum and sum of exponentials of its filled slots.  Returns whether there is one; a
-// class outside [0, V) makes the sum NaN.
+// The teacher of a row, by L lanes: maximum and sum of exponentials of its filled slots, and whether there is one; a class
+// outside [0, V) makes the sum NaN.
 struct Teacher {
-  double m, s;
+  float m;
+  double s;
   bool any;
 };
-__device__ Teacher row_teacher(const DistillParams& P, int64_t row) {
-  const int lane = threadIdx.x & 63;
-  double m = -__builtin_inf();
+template <int L>
+__device__ __forceinline__ Teacher row_teacher(const DistillParams& P, int64_t row) {
+  const int lane = threadIdx.x % L;
+  float m = -__builtin_inff();
   bool any = false, bad = false;
-  for (int j = lane; j < P.top; j += 64) {
+  for (int j = lane; j < P.top; j += L) {
     const int64_t c = slot_class(P, row, j);
+    const float t = load_as_float(P.t, P.t_dtype, row * P.top + j);
     if (c < 0) continue;
-    const double t = (double)load_as_float(P.t, P.t_dtype, row * P.top + j);
     bad |= c >= P.cols || t != t;
-    any |= t != -__builtin_inf();
-    m = fmax(m, t);
+    any |= t != -__builtin_inff();
+    m = __builtin_fmaxf(m, t);
   }
-  m = wave_max(m);
-  bad = __any(bad);
-  any = __any(any) || bad;
+  m = reduce_lanes<L, OpMax>(m);
+  bad = any_lane<L>(bad);
+  any = any_lane<L>(any) || bad;
   double s = 0.0;
-  for (int j = lane; j < P.top; j += 64) {
+  for (int j = lane; j < P.top; j += L) {
     if (slot_class(P, row, j) < 0) continue;
-    s += exp(((double)load_as_float(P.t, P.t_dtype, row * P.top + j) - m) * (double)P.inv_t);
+    s += (double)exp_slot(load_as_float(P.t, P.t_dtype, row * P.top + j), m, P.scale64);
   }
-  s = wave_sum(s);
+  s = sum_lanes<L>(s);
   return {m, bad ? __builtin_nan("") : s, any};
 }
 
-// loss of a row from its softmax statistics, by one wave
-template <typename T>
-__device__ void row_loss(const DistillParams& P, int64_t row, const T* __restrict__ z, float m, float s) {
-  const int lane = threadIdx.x & 63;
-  const Teacher teacher = row_teacher(P, row);
+// Loss of a row from its softmax statistics, by L lanes; keeps the statistics and, without a reduction, stores the loss.
+template <typename T, int L>
+__device__ __forceinline__ double row_loss(const DistillParams& P, int64_t row, const T* __restrict__ z, float m, float s, bool store,
+                                           bool& taught) {
+  const int lane = threadIdx.x % L;
+  const Teacher teacher = row_teacher<L>(P, row);
+  taught = teacher.any;
   double loss = 0.0;
-  if (teacher.any) {
-    const double inv_t = 1.0 / (double)P.temperature;
-    const double log_s = log((double)s), log_ps = log(teacher.s);
-    for (int j = lane; j < P.top; j += 64) {
-      const int64_t c = slot_class(P, row, j);
-      if (c < 0) continue;
-      if (c >= P.cols) {
-        loss = __builtin_nan("");
-        continue;
-      }
-      const double log_p = ((double)load_as_float(P.t, P.t_dtype, row * P.top + j) - teacher.m) * inv_t - log_ps;
-      const double log_q = ((double)(float)z[c] - (double)m) * inv_t - log_s;
-      const double p = exp(log_p);
-      if (p != 0.0) loss += p * (log_p - log_q);
+  const double inv_t = 1.0 / P.temperature, inv_ps = 1.0 / teacher.s;
+  const double log_ratio = log((double)s * inv_ps);  // log p - log q = (t - max t) / T - (z - max z) / T + this
+  for (int j = lane; j < P.top; j += L) {
+    const int64_t c = slot_class(P, row, j);
+    if (c < 0 || !teacher.any) continue;
+    if (c >= P.cols) {
+      loss = __builtin_nan("");
+      continue;
     }
-    loss = wave_sum(loss) * (double)P.temperature * (double)P.temperature;
+    const float t = load_as_float(P.t, P.t_dtype, row * P.top + j);
+    const double p = (double)exp_slot(t, teacher.m, P.scale64) * inv_ps;
+    const double d = (((double)t - (double)teacher.m) - ((double)(float)z[c] - (double)m)) * inv_t + log_ratio;
+    if (p != 0.0) loss += p * d;
   }
-  if (lane == 0) {
+  loss = sum_lanes<L>(loss) * P.temperature * P.temperature;
+  if (lane == 0 && store) {
     if (P.stats) {
       P.stats[2 * row] = m;
       P.stats[2 * row + 1] = s;
     }
-    if (P.reduction == UR_REDUCE_NONE) {
-      P.loss[row] = (float)loss;
-    } else {
-      P.row_loss[row] = (float)loss;
-      P.taught[row] = teacher.any ? 1.0f : 0.0f;
-    }
+    if (P.reduction == UR_REDUCE_NONE) P.loss[row] = (float)loss;
   }
+  return (double)(float)loss;
 }
 
-// one workgroup a row
-template <typename T>
-__global__ void __launch_bounds__(kThreads) k_distill_fwd(const DistillParams P) {
-  __shared__ float part[2][kWaves];
-  const int64_t row = blockIdx.x;
+// Forward, L lanes a row (a row of few classes), kThreads / L rows a workgroup.
+template <typename T, int L>
+__global__ void __launch_bounds__(kThreads) k_distill_fwd_rows(const DistillParams P) {
+  constexpr int R = kThreads / L;
+  __shared__ double part[2][R];
+  const int t = threadIdx.x % L, sub = threadIdx.x / L;
+  const int64_t want = (int64_t)blockIdx.x * R + sub;
+  const bool mine = want < P.rows;
+  const int64_t row = mine ? want : P.rows - 1;  // (idle lanes take part in the exchanges)
   const T* z = static_cast<const T*>(P.z) + row * P.stride;
-  const float scale = P.inv_t * kLog2e;
+  const float scale = P.scale;
   float m, s;
-  row_part<T>(z, 0, P.cols, threadIdx.x, kThreads, scale, m, s);
+  row_part<T, 2>(z, 0, P.cols, t, L, scale, m, s);
+  merge_lanes<L>(m, s, scale);
+  bool taught;
+  const double loss = row_loss<T, L>(P, row, z, m, s, mine, taught);
+  if (P.partial == nullptr) return;
+  if (t == 0) {
+    part[0][sub] = mine ? loss : 0.0;
+    part[1][sub] = mine && taught ? 1.0 : 0.0;
+  }
+  __syncthreads();
+  if (threadIdx.x >= 2) return;
+  double a = 0.0;
+  for (int r = 0; r < R; ++r) a += part[threadIdx.x][r];
+  P.partial[2 * (int64_t)blockIdx.x + threadIdx.x] = a;
+}
+
+// a workgroup's maximum and sum, in every thread
+template <int W>
+__device__ __forceinline__ void merge_waves(float (&part)[2][W], float& m, float& s, float scale) {
   merge_lanes<64>(m, s, scale);
   if ((threadIdx.x & 63) == 0) {
     part[0][threadIdx.x >> 6] = m;
     part[1][threadIdx.x >> 6] = s;
   }
   __syncthreads();
-  if (threadIdx.x >= 64) return;
   m = part[0][0];
   s = part[1][0];
-  for (int w = 1; w < kWaves; ++w) merge(m, s, part[0][w], part[1][w], scale);
-  row_loss<T>(P, row, z, m, s);
+  for (int w = 1; w < W; ++w) merge(m, s, part[0][w], part[1][w], scale);
+}
+
+template <typename T>
+__device__ __forceinline__ void finish_row(const DistillParams& P, int64_t row, const T* z, float m, float s) {
+  bool taught;
+  const double loss = row_loss<T, 64>(P, row, z, m, s, true, taught);
+  if (P.partial && threadIdx.x == 0) {
+    P.partial[2 * row] = loss;
+    P.partial[2 * row + 1] = taught ? 1.0 : 0.0;
+  }
+}
+
+// Forward, one workgroup a row.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_distill_fwd(const DistillParams P) {
+  __shared__ float part[2][kThreads / 64];
+  const int64_t row = blockIdx.x;
+  const T* z = static_cast<const T*>(P.z) + row * P.stride;
+  const float scale = P.scale;
+  float m, s;
+  row_part<T, 4>(z, 0, P.cols, threadIdx.x, kThreads, scale, m, s);
+  merge_waves(part, m, s, scale);
+  if (threadIdx.x < 64) finish_row<T>(P, row, z, m, s);
+}
+
+// Forward, too few rows to fill the chip: a row is split over workgroups, whose maxima and sums a second launch merges.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_distill_split(const DistillParams P) {
+  __shared__ float part[2][kThreads / 64];
+  const int64_t row = blockIdx.y, c0 = (int64_t)blockIdx.x * P.chunk;
+  const T* z = static_cast<const T*>(P.z) + row * P.stride;
+  const float scale = P.scale;
+  float m, s;
+  row_part<T, 1>(z, c0, min(c0 + P.chunk, P.cols), threadIdx.x, kThreads, scale, m, s);
+  merge_waves(part, m, s, scale);
+  if (threadIdx.x == 0) {
+    float* out = P.split_stats + 2 * (row * P.splits + blockIdx.x);
+    out[0] = m;
+    out[1] = s;
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(64) k_distill_join(const DistillParams P) {
+  const int64_t row = blockIdx.x;
+  const float scale = P.scale;
+  float m = -__builtin_inff(), s = 0.0f;
+  for (int i = threadIdx.x; i < P.splits; i += 64) {
+    const float* in = P.split_stats + 2 * (row * P.splits + i);
+    merge(m, s, in[0], in[1], scale);
+  }
+  merge_lanes<64>(m, s, scale);
+  finish_row<T>(P, row, static_cast<const T*>(P.z) + row * P.stride, m, s);
 }
 
 // sum or mean of the rows' losses, in 64 bits and in a fixed order; keeps the factor for the backward
 __global__ void __launch_bounds__(1024) k_distill_reduce(const DistillParams P) {
   __shared__ double part[2][16];
   double a = 0.0, n = 0.0;
-  for (int64_t r = threadIdx.x; r < P.rows; r += 1024) {
-    a += (double)P.row_loss[r];
-    n += (double)P.taught[r];
+#pragma unroll 4
+  for (int64_t r = threadIdx.x; r < P.partials; r += 1024) {
+    a += P.partial[2 * r];
+    n += P.partial[2 * r + 1];
   }
-  a = wave_sum(a);
-  n = wave_sum(n);
+  a = sum_lanes<64>(a);
+  n = sum_lanes<64>(n);
   if ((threadIdx.x & 63) == 0) {
     part[0][threadIdx.x >> 6] = a;
     part[1][threadIdx.x >> 6] = n;
@@ -215,45 +324,77 @@ __global__ void __launch_bounds__(1024) k_distill_reduce(const DistillParams P) 
   if (P.stats) P.stats[2 * P.rows] = (float)factor;
 }
 
-// Backward, one workgroup a row: all of q first, then the teacher's classes are written again with their shares taken off.
-// A class that several slots name gets the sum of their shares, written by the first of them.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) k_distill_bwd(const DistillParams P) {
+// ---- backward: all of q first, then the teacher's classes are written again with their shares taken off.  A class that
+// several slots name gets the sum of their shares, written by the first of them.
+
+// classes and shares of a row's slots, by L lanes; returns 0: no teacher, 1: a teacher, 2: NaN
+template <int L>
+__device__ __forceinline__ int row_shares(const DistillParams& P, int64_t row, int* cls, float* share) {
+  const Teacher teacher = row_teacher<L>(P, row);
+  const float inv_s = (float)(1.0 / teacher.s);
+  for (int j = threadIdx.x % L; j < P.top; j += L) {
+    const int64_t c = slot_class(P, row, j);
+    cls[j] = (c < 0 || c >= P.cols) ? -1 : (int)c;
+    share[j] = c < 0 ? 0.0f : exp_slot(load_as_float(P.t, P.t_dtype, row * P.top + j), teacher.m, P.scale64) * inv_s;
+  }
+  return !teacher.any ? 0 : teacher.s != teacher.s ? 2 : 1;
+}
+
+struct RowGrad {
+  float g, m, inv_s, scale;
+  bool zero;
+  __device__ __forceinline__ float q(float z) const { return exp_diff(z, m, scale) * inv_s; }
+};
+__device__ __forceinline__ RowGrad row_grad(const DistillParams& P, int64_t row, int taught) {
+  RowGrad r;
+  r.g = (float)P.temperature * (P.reduction == UR_REDUCE_NONE ? P.g[row * P.g_stride] : P.g[0] * P.stats[2 * P.rows]);
+  if (taught == 2) r.g = __builtin_nanf("");
+  r.zero = taught == 0;
+  r.m = P.stats[2 * row];
+  r.inv_s = 1.0f / P.stats[2 * row + 1];
+  r.scale = P.scale;
+  return r;
+}
+
+// g q of row elements [c0, c1), threads t, t + n, ...
+template <typename T, int B>
+__device__ __forceinline__ void write_q(const RowGrad& r, const T* __restrict__ z, T* __restrict__ out, int64_t c0, int64_t c1, int t,
+                                        int n) {
   constexpr int N = Elem<T>::kN;
-  __shared__ int cls[kMaxTop];
-  __shared__ float share[kMaxTop];
-  __shared__ int taught;
-  const int64_t row = blockIdx.x;
-  const T* z = static_cast<const T*>(P.z) + row * P.stride;
-  T* out = static_cast<T*>(P.grad) + row * P.cols;
-  const float scale = P.inv_t * kLog2e, m = P.stats[2 * row], s = P.stats[2 * row + 1];
-  if (threadIdx.x < 64) {
-    const Teacher teacher = row_teacher(P, row);
-    for (int j = threadIdx.x; j < P.top; j += 64) {
-      const int64_t c = slot_class(P, row, j);
-      cls[j] = (c < 0 || c >= P.cols) ? -1 : (int)c;
-      const double t = (double)load_as_float(P.t, P.t_dtype, row * P.top + j);
-      share[j] = c < 0 ? 0.0f : (float)(exp((t - teacher.m) * (double)P.inv_t) / teacher.s);
-    }
-    if (threadIdx.x == 0) taught = !teacher.any ? 0 : teacher.s != teacher.s ? 2 : 1;
-  }
-  __syncthreads();
-  float g = P.temperature * (P.reduction == UR_REDUCE_NONE ? P.g[row * P.g_stride] : P.g[0] * P.stats[2 * P.rows]);
-  if (taught == 2) g = __builtin_nanf("");
-  const bool zero = taught == 0;
-  const float inv_s = 1.0f / s;
-  for (int64_t col = (int64_t)threadIdx.x * N; col < P.cols; col += kThreads * N) {
-    const auto v = load16<T>(z, col, P.cols, (T)0.0f);
-    typename Elem<T>::Vec o;
+  using Vec = typename Elem<T>::Vec;
+  int64_t col = c0 + (int64_t)t * N;
+  const int64_t step = (int64_t)n * N;
+  for (; col + (B - 1) * step + N <= c1; col += B * step) {
+    Vec v[B];
 #pragma unroll
-    for (int j = 0; j < N; ++j) o[j] = zero ? (T)0.0f : (T)(g * (exp_diff((float)v[j], m, scale) * inv_s));
-    store16<T>(out, col, P.cols, o);
+    for (int b = 0; b < B; ++b) v[b] = *reinterpret_cast<const Vec*>(z + col + b * step);
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[b][j] = r.zero ? (T)0.0f : (T)(r.g * r.q((float)v[b][j]));
+      __builtin_nontemporal_store(v[b], reinterpret_cast<Vec*>(out + col + b * step));
+    }
   }
-  __syncthreads();
-  if (zero) return;
-  for (int j = threadIdx.x; j < P.top; j += kThreads) {
+  if (col >= c1) return;
+  Vec v[B];
+#pragma unroll
+  for (int b = 0; b < B; ++b) v[b] = load16<T>(z, col + b * step, c1, (T)0.0f);
+#pragma unroll
+  for (int b = 0; b < B; ++b) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[b][j] = r.zero ? (T)0.0f : (T)(r.g * r.q((float)v[b][j]));
+    store16<T>(out, col + b * step, c1, v[b]);
+  }
+}
+
+// the classes of [c0, c1) that slots name, threads t, t + n, ...
+template <typename T>
+__device__ __forceinline__ void write_shares(const DistillParams& P, const RowGrad& r, const T* __restrict__ z, T* __restrict__ out,
+                                             const int* cls, const float* share, int64_t c0, int64_t c1, int t, int n) {
+  if (r.zero) return;
+  for (int j = t; j < P.top; j += n) {
     const int c = cls[j];
-    if (c < 0) continue;
+    if (c < c0 || c >= c1) continue;
     float p = 0.0f;
     bool first = true;
     for (int i = 0; i < P.top; ++i)
@@ -261,12 +402,114 @@ __global__ void __launch_bounds__(kThreads) k_distill_bwd(const DistillParams P)
         first &= i >= j;
         p += share[i];
       }
-    if (first) out[c] = (T)(g * (exp_diff((float)z[c], m, scale) * inv_s - p));
+    if (first) out[c] = (T)(r.g * (r.q((float)z[c]) - p));
   }
 }
 
+// L lanes a row, kThreads / L rows a workgroup; a wave's stores to one place stay in their order
+template <typename T, int L>
+__global__ void __launch_bounds__(kThreads) k_distill_bwd_rows(const DistillParams P) {
+  constexpr int R = kThreads / L;
+  __shared__ int cls[R][kGroupTop];
+  __shared__ float share[R][kGroupTop];
+  const int t = threadIdx.x % L, sub = threadIdx.x / L;
+  const int64_t want = (int64_t)blockIdx.x * R + sub;
+  const bool mine = want < P.rows;
+  const int64_t row = mine ? want : P.rows - 1;
+  const T* z = static_cast<const T*>(P.z) + row * P.stride;
+  T* out = static_cast<T*>(P.grad) + row * P.cols;
+  const RowGrad r = row_grad(P, row, row_shares<L>(P, row, cls[sub], share[sub]));
+  if (mine) write_q<T, 2>(r, z, out, 0, P.cols, t, L);
+  wave_lds_handoff();
+  if (mine) write_shares<T>(P, r, z, out, cls[sub], share[sub], 0, P.cols, t, L);
+}
+
+// a workgroup takes one row or (gridDim.x > 1) a part of one
+template <typename T, int TH>
+__global__ void __launch_bounds__(TH) k_distill_bwd(const DistillParams P) {
+  __shared__ int cls[kMaxTop];
+  __shared__ float share[kMaxTop];
+  __shared__ int taught;
+  const int64_t row = P.splits > 1 ? blockIdx.y : blockIdx.x;
+  const int64_t c0 = P.splits > 1 ? (int64_t)blockIdx.x * P.chunk : 0, c1 = P.splits > 1 ? min(c0 + P.chunk, P.cols) : P.cols;
+  const T* z = static_cast<const T*>(P.z) + row * P.stride;
+  T* out = static_cast<T*>(P.grad) + row * P.cols;
+  if (threadIdx.x < 64) {
+    const int state = row_shares<64>(P, row, cls, share);
+    if (threadIdx.x == 0) taught = state;
+  }
+  __syncthreads();
+  const RowGrad r = row_grad(P, row, taught);
+  write_q<T, 4>(r, z, out, c0, c1, threadIdx.x, TH);
+  __syncthreads();
+  write_shares<T>(P, r, z, out, cls, share, c0, c1, threadIdx.x, TH);
+}
+
+// ---- which kernel a call takes ---------------------------------------------------------------------------------------
+struct DistillPlan {
+  int lanes;         // lanes a row (8, 16, 64), or 0: workgroups
+  int bwd_threads;   // backward: threads of a workgroup that takes a row
+  int splits;        // workgroups a row
+  int64_t chunk;     // classes of a part
+  int64_t partials;  // workgroups that hand a sum to the reduction
+  int64_t ws_bytes;
+};
+
+DistillPlan distill_plan(int64_t rows, int64_t cols, int dtype, int reduction) {
+  DistillPlan p{0, 256, 1, cols, rows, 0};
+  const int n = 16 / dtype_bytes(dtype);
+  const int64_t vecs = ceil_div(cols, n);
+  if (vecs <= 16) p.lanes = 8;
+  else if (vecs <= 64) p.lanes = 16;
+  else if (vecs <= 256) p.lanes = 64;
+  if (p.lanes) {
+    p.partials = ceil_div(rows, kThreads / p.lanes);
+  } else if (rows >= 512) {
+    // Large workgroups walk few rows at a time through memory, which the backward's mixed reads and writes like -- where a
+    // row is a whole number of their batches of 4 vectors a thread, or nearly (8192 x 32768 bf16: 208 us with 1024 threads,
+    // 226 with 512, 240 with 256; 2000 x 20000 fp32, 1.2 batches of 1024 threads: 76, 67, 72).
+    for (int th : {1024, 512})
+      if (p.bwd_threads == 256 && vecs >= 4 * th && (th == 512 || 10 * ceil_div(vecs, 4096) * 4096 <= 11 * vecs)) p.bwd_threads = th;
+  } else {
+    // parts of at least one vector a thread, and about 1024 workgroups
+    const int64_t want = std::min<int64_t>(ceil_div(cols, (int64_t)256 * n), std::max<int64_t>(1, 1024 / rows));
+    p.chunk = ceil_div(ceil_div(cols, want), (int64_t)256 * n) * (256 * n);
+    p.splits = (int)ceil_div(cols, p.chunk);
+  }
+  const int64_t reduce = reduction == UR_REDUCE_NONE ? 0 : p.partials * 16;
+  p.ws_bytes = reduce + (p.splits > 1 ? rows * p.splits * 8 : 0);
+  return p;
+}
+
+template <typename T>
+void launch_fwd(const DistillPlan& p, const DistillParams& P, hipStream_t st) {
+  const unsigned rows = (unsigned)P.rows, groups = (unsigned)p.partials;
+  if (p.lanes == 8) k_distill_fwd_rows<T, 8><<<groups, kThreads, 0, st>>>(P);
+  else if (p.lanes == 16) k_distill_fwd_rows<T, 16><<<groups, kThreads, 0, st>>>(P);
+  else if (p.lanes == 64) k_distill_fwd_rows<T, 64><<<groups, kThreads, 0, st>>>(P);
+  else if (p.splits == 1) k_distill_fwd<T><<<rows, kThreads, 0, st>>>(P);
+  else {
+    k_distill_split<T><<<dim3(p.splits, rows), kThreads, 0, st>>>(P);
+    k_distill_join<T><<<rows, 64, 0, st>>>(P);
+  }
+  if (P.reduction != UR_REDUCE_NONE) k_distill_reduce<<<1, 1024, 0, st>>>(P);
+}
+
+template <typename T>
+void launch_bwd(const DistillPlan& p, const DistillParams& P, hipStream_t st) {
+  const unsigned rows = (unsigned)P.rows;
+  const int lanes = P.top <= kGroupTop ? p.lanes : 0;
+  if (lanes == 8) k_distill_bwd_rows<T, 8><<<(unsigned)ceil_div(P.rows, 32), kThreads, 0, st>>>(P);
+  else if (lanes == 16) k_distill_bwd_rows<T, 16><<<(unsigned)ceil_div(P.rows, 16), kThreads, 0, st>>>(P);
+  else if (lanes == 64) k_distill_bwd_rows<T, 64><<<(unsigned)ceil_div(P.rows, 4), kThreads, 0, st>>>(P);
+  else if (p.splits > 1) k_distill_bwd<T, 256><<<dim3(p.splits, rows), 256, 0, st>>>(P);
+  else if (p.bwd_threads == 256) k_distill_bwd<T, 256><<<rows, 256, 0, st>>>(P);
+  else if (p.bwd_threads == 512) k_distill_bwd<T, 512><<<rows, 512, 0, st>>>(P);
+  else k_distill_bwd<T, 1024><<<rows, 1024, 0, st>>>(P);
+}
+
 int check_common(const void* logits, int64_t stride, int dtype, int64_t rows, int64_t cols, const void* teacher,
-                 int teacher_dtype, const void* index, int index_bytes, int top, float temperature, int reduction) {
+                 int teacher_dtype, const void* index, int index_bytes, int top, double temperature, int reduction) {
   if (!logits || !teacher || !index) return set_error(UR_ERR_INVALID_ARG, "null input pointer");
   if (!known_dtype(dtype) || !known_dtype(teacher_dtype)) return set_error(UR_ERR_INVALID_ARG, "bad dtype");
   if (index_bytes != 4 && index_bytes != 8) return set_error(UR_ERR_INVALID_ARG, "indices have 4 or 8 bytes");
@@ -274,8 +517,8 @@ int check_common(const void* logits, int64_t stride, int dtype, int64_t rows, in
   if (rows > 0x7fffffff || cols > 0x7fffffff) return set_error(UR_ERR_UNSUPPORTED, "rows and cols must be below 2^31");
   if (top > kMaxTop) return set_error(UR_ERR_UNSUPPORTED, "at most %d teacher slots", kMaxTop);
   if (stride < cols && rows > 1) return set_error(UR_ERR_INVALID_ARG, "row stride below the row length");
-  if (!(temperature > 0.0f) || !(temperature - temperature == 0.0f) || !(1.0f / temperature > 0.0f) ||
-      !(1.0f / temperature - 1.0f / temperature == 0.0f))
+  const float scale = (float)(kLog2e / temperature), t32 = (float)temperature;
+  if (!(t32 > 0.0f) || !(t32 - t32 == 0.0f) || !(scale > 0.0f) || !(scale - scale == 0.0f))
     return set_error(UR_ERR_INVALID_ARG, "temperature must be positive and finite, and so must its reciprocal");
   if (reduction != UR_REDUCE_NONE && reduction != UR_REDUCE_SUM && reduction != UR_REDUCE_MEAN)
     return set_error(UR_ERR_INVALID_ARG, "bad reduction %d", reduction);
@@ -283,10 +526,10 @@ int check_common(const void* logits, int64_t stride, int dtype, int64_t rows, in
 }
 
 void fill_common(DistillParams& P, const void* logits, int64_t stride, int64_t rows, int64_t cols, const void* teacher,
-                 int teacher_dtype, const void* index, int index_bytes, int top, float temperature, int reduction) {
+                 int teacher_dtype, const void* index, int index_bytes, int top, double temperature, int reduction) {
   P.z = logits; P.stride = stride; P.rows = rows; P.cols = cols; P.t = teacher; P.t_dtype = teacher_dtype;
   P.index = index; P.index64 = index_bytes == 8; P.top = top; P.temperature = temperature;
-  P.inv_t = 1.0f / temperature; P.reduction = reduction;
+  P.scale64 = kLog2e / temperature; P.scale = (float)P.scale64; P.reduction = reduction;
 }
 
 }  // namespace
@@ -297,37 +540,41 @@ int64_t ur_distill_workspace_bytes(int64_t rows, int64_t cols, int dtype, int re
   if (!known_dtype(dtype)) return set_error(UR_ERR_INVALID_ARG, "bad dtype %d", dtype);
   if (rows <= 0 || cols <= 0 || rows > 0x7fffffff || cols > 0x7fffffff)
     return set_error(UR_ERR_INVALID_ARG, "rows and cols must be positive and below 2^31");
-  return reduction == UR_REDUCE_NONE ? 0 : rows * 2 * 4;
+  return distill_plan(rows, cols, dtype, reduction).ws_bytes;
 }
 
 int ur_distill_forward(const void* logits, int64_t row_stride, int dtype, int64_t rows, int64_t cols, const void* teacher,
-                       int teacher_dtype, const void* index, int index_bytes, int top, float temperature, int reduction,
+                       int teacher_dtype, const void* index, int index_bytes, int top, double temperature, int reduction,
                        float* loss, float* stats, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_common(logits, row_stride, dtype, rows, cols, teacher, teacher_dtype, index, index_bytes, top,
                             temperature, reduction))
     return rc;
   if (!loss) return set_error(UR_ERR_INVALID_ARG, "null output pointer");
-  const size_t need = (size_t)ur_distill_workspace_bytes(rows, cols, dtype, reduction);
+  const DistillPlan plan = distill_plan(rows, cols, dtype, reduction);
+  const size_t need = (size_t)plan.ws_bytes;
   if (workspace_bytes < need || (need && !workspace))
     return set_error(UR_ERR_WORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, need);
+  if (reinterpret_cast<uintptr_t>(workspace) & 7) return set_error(UR_ERR_WORKSPACE, "workspace must be 8-byte aligned");
   DistillParams P{};
   fill_common(P, logits, row_stride, rows, cols, teacher, teacher_dtype, index, index_bytes, top, temperature, reduction);
   P.loss = loss; P.stats = stats;
+  P.splits = plan.splits; P.chunk = plan.chunk; P.partials = plan.partials;
+  char* ws = static_cast<char*>(workspace);
   if (reduction != UR_REDUCE_NONE) {
-    P.row_loss = static_cast<float*>(workspace);
-    P.taught = P.row_loss + rows;
+    P.partial = reinterpret_cast<double*>(ws);
+    ws += plan.partials * 16;
   }
+  if (plan.splits > 1) P.split_stats = reinterpret_cast<float*>(ws);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == UR_F32) k_distill_fwd<float><<<(unsigned)rows, kThreads, 0, st>>>(P);
-  else if (dtype == UR_F16) k_distill_fwd<_Float16><<<(unsigned)rows, kThreads, 0, st>>>(P);
-  else k_distill_fwd<__bf16><<<(unsigned)rows, kThreads, 0, st>>>(P);
-  if (reduction != UR_REDUCE_NONE) k_distill_reduce<<<1, 1024, 0, st>>>(P);
+  if (dtype == UR_F32) launch_fwd<float>(plan, P, st);
+  else if (dtype == UR_F16) launch_fwd<_Float16>(plan, P, st);
+  else launch_fwd<__bf16>(plan, P, st);
   return launch_status("ur_distill_forward");
 }
 
 int ur_distill_backward(const float* grad_loss, int64_t grad_stride, const void* logits, int64_t row_stride, int dtype,
                         int64_t rows, int64_t cols, const void* teacher, int teacher_dtype, const void* index,
-                        int index_bytes, int top, float temperature, int reduction, const float* stats,
+                        int index_bytes, int top, double temperature, int reduction, const float* stats,
                         void* grad_logits, void* stream) {
   if (int rc = check_common(logits, row_stride, dtype, rows, cols, teacher, teacher_dtype, index, index_bytes, top,
                             temperature, reduction))
@@ -337,10 +584,12 @@ int ur_distill_backward(const float* grad_loss, int64_t grad_stride, const void*
   DistillParams P{};
   fill_common(P, logits, row_stride, rows, cols, teacher, teacher_dtype, index, index_bytes, top, temperature, reduction);
   P.g = grad_loss; P.g_stride = grad_stride; P.stats = const_cast<float*>(stats); P.grad = grad_logits;
+  const DistillPlan plan = distill_plan(rows, cols, dtype, reduction);
+  P.splits = plan.splits; P.chunk = plan.chunk;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == UR_F32) k_distill_bwd<float><<<(unsigned)rows, kThreads, 0, st>>>(P);
-  else if (dtype == UR_F16) k_distill_bwd<_Float16><<<(unsigned)rows, kThreads, 0, st>>>(P);
-  else k_distill_bwd<__bf16><<<(unsigned)rows, kThreads, 0, st>>>(P);
+  if (dtype == UR_F32) launch_bwd<float>(plan, P, st);
+  else if (dtype == UR_F16) launch_bwd<_Float16>(plan, P, st);
+  else launch_bwd<__bf16>(plan, P, st);
   return launch_status("ur_distill_backward");
 }
 

@@ -17,6 +17,7 @@ BLEND_HARD, BLEND_CLIP_INSIDE, BLEND_SIGMOID, BLEND_SOFTMAX = 0, 1, 2, 3
 _lib = None
 
 _vp, _i, _i64, _f, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
+_d = ctypes.c_double
 _F3 = ctypes.c_float * 3
 
 _SIGNATURES = {
@@ -59,8 +60,8 @@ _SIGNATURES = {
     "ur_layer_norm_backward": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i, _i, _i64, _i64, _vp, _vp, _vp, _vp, _sz,
                                     _vp]),
     "ur_distill_workspace_bytes": (_i64, [_i64, _i64, _i, _i]),
-    "ur_distill_forward": (_i, [_vp, _i64, _i, _i64, _i64, _vp, _i, _vp, _i, _i, _f, _i, _vp, _vp, _vp, _sz, _vp]),
-    "ur_distill_backward": (_i, [_vp, _i64, _vp, _i64, _i, _i64, _i64, _vp, _i, _vp, _i, _i, _f, _i, _vp, _vp, _vp]),
+    "ur_distill_forward": (_i, [_vp, _i64, _i, _i64, _i64, _vp, _i, _vp, _i, _i, _d, _i, _vp, _vp, _vp, _sz, _vp]),
+    "ur_distill_backward": (_i, [_vp, _i64, _vp, _i64, _i, _i64, _i64, _vp, _i, _vp, _i, _i, _d, _i, _vp, _vp, _vp]),
     "ur_route_workspace_bytes": (_i64, [_i64, _i]),
     "ur_route_forward": (_i, [_vp, _i64, _i, _vp, _i64, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _vp, _vp, _vp, _sz, _vp]),
     "ur_route_backward": (_i, [_vp, _vp, _i64, _i, _i64, _i, _vp, _vp, _i, _i, _i, _f, _vp, _vp]),
