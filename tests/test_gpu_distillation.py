@@ -292,6 +292,14 @@ def test_two_backwards_changed_inputs_streams_and_repeats():
     y.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+    loss = distill_top_logits(x, t, i)
+    loss.backward(inputs=[x])
+    with pytest.raises(RuntimeError, match="second time"):
+        loss.backward(inputs=[x])
+    g2 = torch.autograd.grad(distill_top_logits(x, t, i), x, create_graph=True)[0]
+    assert torch.equal(g2.detach(), first)
+    with pytest.raises(RuntimeError, match="twice"):
+        g2.float().sum().backward()
     assert not distill_top_logits(z, t.clone().requires_grad_(True), i).requires_grad   # the teacher gets none
 
 

@@ -159,7 +159,7 @@ def test_rows_behind_and_beside_the_input_are_left_alone():
     big = torch.full((11, 64), 7.0, device="cuda", dtype=torch.bfloat16)
     big[1:10, 3:53] = x
     before = big.clone()
-    y, _ = native.layer_norm_forward(big[1:10, 3:53], None, None, 1e-5, False)
+    y, _ = native.nodes().layer_norm_forward(big[1:10, 3:53], None, None, 1e-5, False)
     assert torch.equal(big, before)
     check(y, reference(x, None, None, 1e-5)["y"], "y")
 
@@ -254,6 +254,14 @@ def test_two_backwards_and_changed_inputs():
     z.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward(dy)
+    y = layer_norm(x, w, b)
+    torch.autograd.grad(y, x, dy)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, x, dy)
+    g = torch.autograd.grad(layer_norm(x, w, b), x, dy, create_graph=True)[0]
+    assert torch.equal(g.detach(), first)
+    with pytest.raises(RuntimeError, match="twice"):
+        g.sum().backward()
 
 
 def test_same_bits_every_time_and_on_another_stream():

@@ -336,6 +336,15 @@ def test_two_backwards_changed_inputs_streams_and_repeats():
     y.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         r.weights.sum().backward()
+    r = route_candidates(x, 8, **kw)
+    r.weights.data.mul_(1.0)                              # (.data: not counted as a change)
+    torch.autograd.grad(r.weights, x, dw)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(r.weights, x, dw)
+    g2 = torch.autograd.grad(route_candidates(x, 8, **kw).weights, x, dw, create_graph=True)[0]
+    assert torch.equal(g2.detach(), g)
+    with pytest.raises(RuntimeError, match="twice"):
+        g2.float().sum().backward()
 
 
 @pytest.mark.parametrize("rows,cands,k", [(32, 6, 2), (600, 256, 8)])

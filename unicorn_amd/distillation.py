@@ -11,9 +11,6 @@ leaves where nothing was eligible); several slots may name one class; a row with
 a NaN among the row's logits or teacher logits does; -inf rules a class or slot out (a class the teacher wants
 that the student rules out makes the loss infinite, its gradient stays finite).
 """
-from torch.autograd import Function
-from torch.autograd.function import once_differentiable
-
 import torch
 
 from . import native
@@ -22,28 +19,13 @@ MAX_SLOTS = 1024
 REDUCTIONS = {"none": native.REDUCE_NONE, "sum": native.REDUCE_SUM, "mean": native.REDUCE_MEAN}
 
 
-class _Distill(Function):
-    @staticmethod
-    def forward(ctx, logits, teacher, index, temperature, reduction):
-        loss, stats = native.distill_forward(logits, teacher, index, temperature, reduction, True)
-        ctx.save_for_backward(logits, teacher, index, stats)
-        ctx.cfg = (temperature, reduction)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_loss):
-        logits, teacher, index, stats = ctx.saved_tensors
-        return native.distill_backward(grad_loss, logits, teacher, index, *ctx.cfg, stats), None, None, None, None
-
-
 def distill_top_logits(logits, teacher_logits, teacher_index, temperature=1.0, reduction="mean"):
     """logits (..., V); teacher_logits, teacher_index (..., k) with the same leading dimensions.  -> float32: one value, or
     one per row with reduction="none"."""
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits need a last dimension of at least 1, got shape {tuple(logits.shape)}")
-    native.dtype_code(logits, "logits")
-    native.dtype_code(teacher_logits, "teacher_logits")
+    native.check_type(logits, "logits")
+    native.check_type(teacher_logits, "teacher_logits")
     if teacher_index.dtype is not torch.int64 and teacher_index.dtype is not torch.int32:
         raise ValueError(f"teacher_index must be int32 or int64, got {teacher_index.dtype}")
     if teacher_logits.dim() < 1 or teacher_logits.shape != teacher_index.shape or teacher_logits.shape[-1] < 1 \
@@ -59,6 +41,5 @@ def distill_top_logits(logits, teacher_logits, teacher_index, temperature=1.0, r
         raise ValueError(f"temperature must be between 1e-30 and 1e30, got {temperature}")
     teacher_logits = teacher_logits.detach().contiguous()
     teacher_index = teacher_index.contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _Distill.apply(logits, teacher_logits, teacher_index, temperature, REDUCTIONS[reduction])
-    return native.distill_forward(logits, teacher_logits, teacher_index, temperature, REDUCTIONS[reduction], False)[0]
+    native.on_gpu(logits)
+    return native.nodes().distill(logits, teacher_logits, teacher_index, temperature, REDUCTIONS[reduction])

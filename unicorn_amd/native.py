@@ -616,157 +616,38 @@ def selftest_division(n, seed=0, device="cuda"):
 
 
 # ---- operators of the networks around the renderer (rows of fp32 / fp16 / bf16) -------------------------------------
-F32, F16, BF16 = 0, 1, 2  # UR_F32, UR_F16, UR_BF16
-_DTYPE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+ROW_TYPES = frozenset((torch.float32, torch.float16, torch.bfloat16))
 
 
-def dtype_code(t, what="tensor"):
-    code = _DTYPE.get(t.dtype)
-    if code is None:
+def check_type(t, what):
+    if t.dtype not in ROW_TYPES:
         raise ValueError(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
-    return code
 
 
-def same_device(t, *others):
-    """`t` lives on a GPU and so do the others, on the same one"""
+def on_gpu(t):
     if not t.is_cuda:
         _ptr(t)
-    for o in others:
-        if o is not None and o.device != t.device:
-            raise ValueError(f"tensors must be on one device: {t.device} and {o.device}")
 
 
-def rows_of(t):
-    """(tensor, rows, row stride) of a tensor read as rows of its last dimension: as it lies where its rows are dense and
-    evenly spaced without overlap (any stride between them), a contiguous copy otherwise"""
-    D = t.shape[-1]
-    if t.is_contiguous():
-        return t, t.numel() // D if D else 0, D
-    if D == 1 or t.stride(-1) == 1:
-        flat = t
-        if t.dim() != 2:
-            try:
-                flat = t.view(-1, D)
-            except RuntimeError:
-                flat = None
-        if flat is not None and (flat.shape[0] <= 1 or flat.stride(0) >= D):
-            return flat, flat.shape[0], max(flat.stride(0), D)
-    t = t.contiguous()
-    return t, t.numel() // D if D else 0, D
+_nodes = None
+NODES_PATH = os.path.join(_HERE, "lib", "unicorn_autograd.so")
 
 
-def _ws(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-
-
-def layer_norm_forward(x, weight, bias, eps, need_stats):
-    """x (..., D) -> y (x's shape, contiguous), mean, rstd (f32, one per row; None unless asked for)"""
-    same_device(x, weight, bias)
-    code = dtype_code(x)
-    pcode = code if weight is None and bias is None else dtype_code(weight if weight is not None else bias)
-    x, M, stride = rows_of(x)
-    D = x.shape[-1]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, M), dtype=torch.float32, device=x.device) if need_stats else None
-    if M:
-        n = _sized("ur_layer_norm_workspace_bytes", M, D, code, 0)
-        ws = _ws(n, x.device)
-        p = stats.data_ptr() if need_stats else None
-        _call("ur_layer_norm_forward", x, x.data_ptr(), stride, _ptr(weight, None, True), _ptr(bias, None, True), code,
-              pcode, M, D, eps, y.data_ptr(), p, p + 4 * M if need_stats else None,
-              ws.data_ptr() if n else None, n, _stream(x))
-    return y, stats
-
-
-def layer_norm_backward(grad_y, x, weight, param_dtype, stats, need_x, need_weight, need_bias):
-    """-> grad_x (x's shape), grad_weight, grad_bias (D); None where not asked for"""
-    code = dtype_code(x)
-    grad_y, M, gstride = rows_of(grad_y)
-    x, _, stride = rows_of(x)
-    D = x.shape[-1]
-    dev = x.device
-    if not M:
-        zeros = lambda need: torch.zeros(D, dtype=param_dtype, device=dev) if need else None
-        return (torch.empty_like(x) if need_x else None), zeros(need_weight), zeros(need_bias)
-    gx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-    gw = torch.empty(D, dtype=param_dtype, device=dev) if need_weight else None
-    gb = torch.empty(D, dtype=param_dtype, device=dev) if need_bias else None
-    n = _sized("ur_layer_norm_workspace_bytes", M, D, code, 1)
-    ws = _ws(n, dev)
-    p = stats.data_ptr()
-    _call("ur_layer_norm_backward", x, grad_y.data_ptr(), gstride, x.data_ptr(), stride, _ptr(weight, None, True), p,
-          p + 4 * M, code, _DTYPE[param_dtype] if param_dtype is not None else code, M, D, _ptr(gx, None, True),
-          _ptr(gw, None, True), _ptr(gb, None, True), ws.data_ptr() if n else None, n, _stream(x))
-    return gx, gw, gb
-
-
-def route_forward(logits, bias, top_k, score, groups, top_groups, group_score, renormalize, scale):
-    """logits (..., E) -> weights f32 (..., k), indices i64 (..., k), counts i32 (E)"""
-    same_device(logits, bias)
-    code = dtype_code(logits)
-    x, M, stride = rows_of(logits)
-    dev, E = x.device, x.shape[-1]
-    shape = logits.shape[:-1] + (top_k,)
-    weights = torch.empty(shape, dtype=torch.float32, device=dev)
-    indices = torch.empty(shape, dtype=torch.int64, device=dev)
-    if not M:
-        return weights, indices, torch.zeros(E, dtype=torch.int32, device=dev)
-    counts = torch.empty(E, dtype=torch.int32, device=dev)
-    n = _sized("ur_route_workspace_bytes", M, E)
-    ws = _ws(n, dev)
-    _call("ur_route_forward", x, x.data_ptr(), stride, code, _ptr(bias, torch.float32, True), M, E, top_k, score, groups,
-          top_groups, group_score, renormalize, scale, weights.data_ptr(), indices.data_ptr(), counts.data_ptr(),
-          ws.data_ptr() if n else None, n, _stream(x))
-    return weights, indices, counts
-
-
-def route_backward(grad_weights, logits, weights, indices, score, renormalize, scale):
-    """-> grad of logits (their shape and type)"""
-    code = dtype_code(logits)
-    x, M, stride = rows_of(logits)
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=x.device)
-    if M:
-        _call("ur_route_backward", x, _ptr(grad_weights.contiguous(), torch.float32), x.data_ptr(), stride, code, M,
-              x.shape[-1], _ptr(weights, torch.float32), _ptr(indices, torch.int64), indices.shape[-1], score, renormalize,
-              scale, grad.data_ptr(), _stream(x))
-    return grad
+def nodes():
+    """The C++ module of the operators' autograd nodes (csrc/ur_autograd.cpp), bound to the library loaded here: layer_norm,
+    route, distill, and each one's `_forward` / `_backward` without a graph.  Arguments are checked by the Python layer."""
+    global _nodes
+    if _nodes is None:
+        if not os.path.exists(NODES_PATH):
+            raise RuntimeError(f"{NODES_PATH} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'`. "
+                               f"There is no CPU/PyTorch fallback.")
+        import importlib.util
+        spec = importlib.util.spec_from_file_location("unicorn_autograd", NODES_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind({name: ctypes.cast(getattr(lib(), name), _vp).value for name in _SIGNATURES})
+        _nodes = module
+    return _nodes
 
 
 REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = 0, 1, 2  # UR_REDUCE_*
-
-
-def distill_forward(logits, teacher, index, temperature, reduction, need_stats):
-    """logits (..., V), teacher (..., k), index i32 / i64 (..., k) -> loss f32 (rows' shape, or one value), stats"""
-    same_device(logits, teacher, index)
-    code = dtype_code(logits)
-    x, M, stride = rows_of(logits)
-    dev, V = x.device, x.shape[-1]
-    per_row = reduction == REDUCE_NONE
-    loss = torch.empty(logits.shape[:-1] if per_row else (), dtype=torch.float32, device=dev)
-    stats = torch.empty(2 * M + 1, dtype=torch.float32, device=dev) if need_stats else None
-    if not M:
-        return (loss if per_row else loss.zero_()), stats
-    n = _sized("ur_distill_workspace_bytes", M, V, code, reduction)
-    ws = _ws(n, dev)
-    _call("ur_distill_forward", x, x.data_ptr(), stride, code, M, V, _ptr(teacher), dtype_code(teacher), _ptr(index),
-          index.element_size(), index.shape[-1], temperature, reduction, loss.data_ptr(), _ptr(stats, None, True),
-          ws.data_ptr() if n else None, n, _stream(x))
-    return loss, stats
-
-
-def distill_backward(grad_loss, logits, teacher, index, temperature, reduction, stats):
-    """-> grad of logits (their shape and type)"""
-    code = dtype_code(logits)
-    x, M, stride = rows_of(logits)
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=x.device)
-    if M:
-        g = grad_loss
-        if reduction == REDUCE_NONE and g.dim() != 1:
-            g = g.reshape(-1)
-        gstride = g.stride(0) if g.dim() else 0
-        if gstride < 0:
-            g, gstride = g.contiguous(), 1
-        _call("ur_distill_backward", x, g.data_ptr(), gstride, x.data_ptr(), stride, code, M, x.shape[-1], _ptr(teacher),
-              dtype_code(teacher), _ptr(index), index.element_size(), index.shape[-1], temperature, reduction,
-              stats.data_ptr(), grad.data_ptr(), _stream(x))
-    return grad

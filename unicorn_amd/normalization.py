@@ -11,34 +11,15 @@ No rows give an empty result and zero parameter gradients.  A row that holds an 
 """
 import torch
 from torch import nn
-from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import native
-
-
-class _LayerNorm(Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, stats = native.layer_norm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, stats)
-        param = weight if weight is not None else bias
-        ctx.param_dtype = None if param is None else param.dtype
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_y):
-        x, weight, stats = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        return native.layer_norm_backward(grad_y, x, weight, ctx.param_dtype, stats, need_x, need_w, need_b) + (None,)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Normalises the last dimension of x.  -> a contiguous tensor of x's shape and type."""
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"layer_norm needs a last dimension of at least 1, got shape {tuple(x.shape)}")
-    native.dtype_code(x, "x")
+    native.check_type(x, "x")
     dtype = None
     for name, p in (("weight", weight), ("bias", bias)):
         if p is None:
@@ -52,12 +33,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         dtype = p.dtype
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
+    native.on_gpu(x)
     weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
     bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
-        return _LayerNorm.apply(x, weight, bias, eps)
-    return native.layer_norm_forward(x, weight, bias, eps, False)[0]
+    return native.nodes().layer_norm(x, weight, bias, eps)
 
 
 class LayerNorm(nn.Module):

@@ -20,8 +20,6 @@ is chosen does.
 from typing import NamedTuple
 
 import torch
-from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import native
 
@@ -36,31 +34,12 @@ class Routing(NamedTuple):
     counts: torch.Tensor
 
 
-class _Route(Function):
-    @staticmethod
-    def forward(ctx, logits, bias, cfg):
-        weights, indices, counts = native.route_forward(logits, bias, *cfg)
-        ctx.save_for_backward(logits, weights, indices)
-        ctx.cfg = (cfg[1], cfg[5], cfg[6])
-        ctx.mark_non_differentiable(indices, counts)
-        ctx.set_materialize_grads(False)
-        return weights, indices, counts
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_weights, _indices, _counts):
-        if grad_weights is None:
-            return None, None, None
-        logits, weights, indices = ctx.saved_tensors
-        return native.route_backward(grad_weights, logits, weights, indices, *ctx.cfg), None, None
-
-
 def route_candidates(logits, top_k, bias=None, score="softmax", groups=1, top_groups=1, group_score="max",
                      renormalize=True, scale=1.0):
     """Chooses `top_k` candidates of every row of logits (..., E).  -> Routing(weights, indices, counts)."""
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits need a last dimension of at least 1, got shape {tuple(logits.shape)}")
-    native.dtype_code(logits, "logits")
+    native.check_type(logits, "logits")
     E = logits.shape[-1]
     if score not in SCORES:
         raise ValueError(f"score must be one of {sorted(SCORES)}, got {score!r}")
@@ -83,11 +62,9 @@ def route_candidates(logits, top_k, bias=None, score="softmax", groups=1, top_gr
             raise ValueError(f"bias must be float32 of shape ({E},), got {bias.dtype} {tuple(bias.shape)}")
         bias = bias.detach()
         bias = bias if bias.is_contiguous() else bias.contiguous()
-    cfg = (int(top_k), SCORES[score], int(groups), int(top_groups), GROUP_SCORES[group_score], int(bool(renormalize)),
-           scale)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return Routing(*_Route.apply(logits, bias, cfg))
-    return Routing(*native.route_forward(logits, bias, *cfg))
+    native.on_gpu(logits)
+    return Routing(*native.nodes().route(logits, bias, top_k, SCORES[score], groups, top_groups, GROUP_SCORES[group_score],
+                                         bool(renormalize), scale))
 
 
 @torch.no_grad()
