@@ -38,24 +38,59 @@ struct LnParams {
   void* db;
 };
 
-// parameters of kN consecutive columns as floats (1 / 0 behind the row's end or without a parameter)
+// A thread's vector of a row.  The vector that would reach over the row's end is moved back to end with the row: its first
+// `skip` elements belong to the vector before it and are left out of sums (and stored twice, with the same value), so that no
+// access is partial.  A vector wholly behind the end has skip >= kN.
 template <typename T>
-__device__ __forceinline__ void load_params(const void* p, int dtype, int64_t col, int64_t cols, float missing,
-                                            float (&out)[Elem<T>::kN]) {
+struct Span {
+  int at, skip;
+  __device__ __forceinline__ Span(int vec, int cols) {
+    const int over = (vec + 1) * Elem<T>::kN - cols;
+    skip = min(max(over, 0), Elem<T>::kN);
+    at = min(vec * Elem<T>::kN, cols - Elem<T>::kN);
+  }
+};
+
+// rows shorter than a vector are read element by element: `at` is negative there
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::Vec load_span(const T* __restrict__ row, int at) {
+  if (at >= 0) return *reinterpret_cast<const typename Elem<T>::Vec*>(row + at);
+  typename Elem<T>::Vec v;
+#pragma unroll
+  for (int j = 0; j < Elem<T>::kN; ++j) v[j] = at + j >= 0 ? row[at + j] : (T)0.0f;
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store_span(T* __restrict__ row, int at, typename Elem<T>::Vec v) {
+  if (at >= 0) {
+    *reinterpret_cast<typename Elem<T>::Vec*>(row + at) = v;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < Elem<T>::kN; ++j)
+    if (at + j >= 0) row[at + j] = v[j];
+}
+
+// parameters of a vector's columns as floats
+template <typename T>
+__device__ __forceinline__ void load_params(const void* p, int dtype, int64_t at, float missing, float (&out)[Elem<T>::kN]) {
   constexpr int N = Elem<T>::kN;
   if (p == nullptr) {
 #pragma unroll
     for (int j = 0; j < N; ++j) out[j] = missing;
-  } else if (dtype == UR_F32) {
-    const float* f = static_cast<const float*>(p);
+  } else if (dtype == UR_F32 && N == 8 && at >= 0) {
+    const f32x4* f = reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + at);
+    const f32x4 lo = f[0], hi = f[1];
 #pragma unroll
-    for (int k = 0; k < N; k += 4) {
-      const f32x4 v = load16<float>(f, col + k, cols, missing);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) out[k + j] = v[j];
+    for (int j = 0; j < 4; ++j) {
+      out[j] = lo[j];
+      out[(4 + j) % N] = hi[j];
     }
+  } else if (dtype == UR_F32 && N == 8) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) out[j] = at + j >= 0 ? static_cast<const float*>(p)[at + j] : missing;
   } else {
-    const auto v = load16<T>(static_cast<const T*>(p), col, cols, (T)missing);
+    const auto v = load_span<T>(static_cast<const T*>(p), at);
 #pragma unroll
     for (int j = 0; j < N; ++j) out[j] = (float)v[j];
   }
@@ -66,30 +101,32 @@ template <typename T, int TPR, int NV>
 __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR) k_ln_fwd(const LnParams P) {
   constexpr int N = Elem<T>::kN, kRows = TPR <= 64 ? 256 / TPR : 1;
   __shared__ float part[2][TPR <= 64 ? 1 : TPR / 64];
-  const int t = threadIdx.x % TPR;
+  const int t = threadIdx.x % TPR, cols = (int)P.cols;
   const int64_t want = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
   const bool mine = want < P.rows;
   const int64_t row = mine ? want : P.rows - 1;  // (idle lanes take part in the lane exchanges)
   const T* x = static_cast<const T*>(P.x) + row * P.x_stride;
   typename Elem<T>::Vec v[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) v[i] = load16<T>(x, (int64_t)(t + i * TPR) * N, P.cols, (T)0.0f);
+  for (int i = 0; i < NV; ++i) v[i] = load_span<T>(x, Span<T>(t + i * TPR, cols).at);
   float s[1] = {0.0f};
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    const int skip = Span<T>(t + i * TPR, cols).skip;
 #pragma unroll
-    for (int j = 0; j < N; ++j) s[0] += (float)v[i][j];
+    for (int j = 0; j < N; ++j) s[0] += j >= skip ? (float)v[i][j] : 0.0f;
+  }
   sum_threads<TPR, 1>(s, part[0]);
   const float inv_d = 1.0f / (float)P.cols;
   const float mean = s[0] * inv_d;
   float q[1] = {0.0f};
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int64_t left = P.cols - (int64_t)(t + i * TPR) * N;
+    const int skip = Span<T>(t + i * TPR, cols).skip;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const float d = (float)v[i][j] - mean;
-      if (j < left) q[0] = __builtin_fmaf(d, d, q[0]);
+      const float d = j >= skip ? (float)v[i][j] - mean : 0.0f;
+      q[0] = __builtin_fmaf(d, d, q[0]);
     }
   }
   sum_threads<TPR, 1>(q, part[1]);
@@ -101,123 +138,170 @@ __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR) k_ln_fwd(const LnParams
   T* y = static_cast<T*>(P.y) + row * P.cols;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int64_t col = (int64_t)(t + i * TPR) * N;
-    if (col >= P.cols || !mine) continue;
+    const Span<T> at(t + i * TPR, cols);
+    if (at.skip >= N || !mine) continue;
     float w[N], b[N];
-    load_params<T>(P.w, P.param_dtype, col, P.cols, 1.0f, w);
-    load_params<T>(P.b, P.param_dtype, col, P.cols, 0.0f, b);
+    load_params<T>(P.w, P.param_dtype, at.at, 1.0f, w);
+    load_params<T>(P.b, P.param_dtype, at.at, 0.0f, b);
     typename Elem<T>::Vec o;
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] = (T)__builtin_fmaf(((float)v[i][j] - mean) * rstd, w[j], b[j]);
-    store16<T>(y, col, P.cols, o);
+    store_span<T>(y, at.at, o);
   }
 }
 
-// Workgroups walk over the rows; a thread keeps its columns' sums of dy h and dy in registers on the way.  At the end
-// the workgroup's groups of threads are added in order and stored as one row of partial sums, which k_ln_param_sums
-// adds up: no atomics, the same result every time.
+// Backward: workgroups of 1024 threads, 1024 / TPR rows at a time, walk over the rows with the next rows' loads in flight; a
+// thread keeps its columns' weights and their sums of dy h and dy in registers on the way.  At the end the groups of threads
+// are added in order and stored as one row of partial sums, which k_ln_param_sums adds up: no atomics, the same result
+// every time.  Large workgroups, one for each CU, because every one of them leaves 2 D floats behind.
+constexpr int kBwdThreads = 1024, kBwdBlocks = 256;
+
+// adds up what lanes TPR, 2 TPR, ... apart hold
+template <int TPR>
+__device__ __forceinline__ float sum_subgroups(float v) {
+  if constexpr (TPR <= 8) v += __uint_as_float(dpp32<0x128>(__float_as_uint(v)));  // (rotation by 8 of 16 lanes)
+  if constexpr (TPR <= 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if constexpr (TPR <= 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return v;
+}
+
 template <typename T, int TPR, int NV>
-__global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR) k_ln_bwd(const LnParams P) {
-  constexpr int N = Elem<T>::kN, kRows = TPR <= 64 ? 256 / TPR : 1;
-  __shared__ float part[2][TPR <= 64 ? 1 : 2 * (TPR / 64)];
-  __shared__ float sums[kRows > 1 ? 2 * TPR * NV * N : 1];
-  const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
-  float aw[NV][N], ab[NV][N];
+__global__ void __launch_bounds__(kBwdThreads) k_ln_bwd(const LnParams P) {
+  using Vec = typename Elem<T>::Vec;
+  constexpr int N = Elem<T>::kN, kRows = kBwdThreads / TPR, kWavesPerRow = TPR > 64 ? TPR / 64 : 1;
+  constexpr int kSets = TPR < 64 ? kBwdThreads / 64 : kRows;  // of sums, once a wave's groups are added
+  __shared__ float part[2][kBwdThreads / 64][2];
+  __shared__ float sums[kSets > 1 ? kSets : 1][kSets > 1 ? 2 * TPR * N : 1];
+  const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, wave = threadIdx.x >> 6, cols = (int)P.cols;
+  float w[NV][N], aw[NV][N], ab[NV][N];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    load_params<T>(P.w, P.param_dtype, Span<T>(t + i * TPR, cols).at, 1.0f, w[i]);
 #pragma unroll
     for (int j = 0; j < N; ++j) aw[i][j] = ab[i][j] = 0.0f;
+  }
   const float inv_d = 1.0f / (float)P.cols;
   const int64_t groups = (P.rows + kRows - 1) / kRows;
-  int flip = 0;
-  for (int64_t rg = blockIdx.x; rg < groups; rg += gridDim.x) {
-    const int64_t want = rg * kRows + sub;
-    const bool mine = want < P.rows;
-    const int64_t row = mine ? want : P.rows - 1;
+  Vec v[NV], u[NV];
+  float mean, rstd;
+  const auto fetch = [&](int64_t rg, Vec (&xv)[NV], Vec (&dv)[NV], float& mu, float& rs) {
+    const int64_t row = min(rg * kRows + sub, P.rows - 1);
     const T* x = static_cast<const T*>(P.x) + row * P.x_stride;
     const T* dy = static_cast<const T*>(P.dy) + row * P.dy_stride;
-    typename Elem<T>::Vec v[NV], u[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      v[i] = load16<T>(x, (int64_t)(t + i * TPR) * N, P.cols, (T)0.0f);
-      u[i] = load16<T>(dy, (int64_t)(t + i * TPR) * N, P.cols, (T)0.0f);
+      const int at = Span<T>(t + i * TPR, cols).at;
+      xv[i] = load_span<T>(x, at);
+      dv[i] = load_span<T>(dy, at);
     }
-    const float mean = P.mean[row], rstd = P.rstd[row];
+    mu = P.mean[row];
+    rs = P.rstd[row];
+  };
+  fetch(blockIdx.x, v, u, mean, rstd);
+  int flip = 0;
+  for (int64_t rg = blockIdx.x; rg < groups; rg += gridDim.x) {
+    Vec v2[NV], u2[NV];
+    float mean2, rstd2;
+    fetch(min(rg + gridDim.x, groups - 1), v2, u2, mean2, rstd2);
+    const bool mine = rg * kRows + sub < P.rows;
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int64_t col = (int64_t)(t + i * TPR) * N;
-      if (col >= P.cols) continue;
-      float w[N];
-      load_params<T>(P.w, P.param_dtype, col, P.cols, 1.0f, w);
+      const int skip = mine ? Span<T>(t + i * TPR, cols).skip : N;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const float h = ((float)v[i][j] - mean) * rstd, d = (float)u[i][j], g = d * w[j];
-        if (col + j < P.cols) {  // (a column behind the end has dy = 0, but its h may be infinite)
+        const float h = ((float)v[i][j] - mean) * rstd, d = (float)u[i][j], g = d * w[i][j];
+        if (j >= skip) {
           s[0] += g;
           s[1] = __builtin_fmaf(g, h, s[1]);
-          if (mine) {
-            aw[i][j] = __builtin_fmaf(d, h, aw[i][j]);
-            ab[i][j] += d;
-          }
+          aw[i][j] = __builtin_fmaf(d, h, aw[i][j]);
+          ab[i][j] += d;
         }
       }
     }
-    sum_threads<TPR, 2>(s, part[flip]);
-    flip ^= 1;  // (the next row's partial sums go to the other half: one barrier a row is enough)
-    if (P.y == nullptr || !mine) continue;
-    const float c1 = s[0] * inv_d, c2 = s[1] * inv_d;
-    T* dx = static_cast<T*>(P.y) + row * P.cols;
+    s[0] = reduce_lanes<(TPR < 64 ? TPR : 64), OpSum>(s[0]);
+    s[1] = reduce_lanes<(TPR < 64 ? TPR : 64), OpSum>(s[1]);
+    if constexpr (TPR > 64) {
+      if ((threadIdx.x & 63) == 0) {
+        part[flip][wave][0] = s[0];
+        part[flip][wave][1] = s[1];
+      }
+      __syncthreads();
+      s[0] = s[1] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kWavesPerRow; ++k) {
+        s[0] += part[flip][sub * kWavesPerRow + k][0];
+        s[1] += part[flip][sub * kWavesPerRow + k][1];
+      }
+      flip ^= 1;  // (the next row's partial sums go to the other half: one barrier a row is enough)
+    }
+    if (P.y != nullptr && mine) {
+      const float c1 = s[0] * inv_d, c2 = s[1] * inv_d;
+      T* dx = static_cast<T*>(P.y) + (rg * kRows + sub) * P.cols;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const Span<T> at(t + i * TPR, cols);
+        if (at.skip >= N) continue;
+        Vec o;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const float h = ((float)v[i][j] - mean) * rstd, g = (float)u[i][j] * w[i][j];
+          o[j] = (T)(rstd * (g - c1 - h * c2));
+        }
+        store_span<T>(dx, at.at, o);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int64_t col = (int64_t)(t + i * TPR) * N;
-      if (col >= P.cols) continue;
-      float w[N];
-      load_params<T>(P.w, P.param_dtype, col, P.cols, 1.0f, w);
-      typename Elem<T>::Vec o;
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float h = ((float)v[i][j] - mean) * rstd, g = (float)u[i][j] * w[j];
-        o[j] = (T)(rstd * (g - c1 - h * c2));
-      }
-      store16<T>(dx, col, P.cols, o);
+      v[i] = v2[i];
+      u[i] = u2[i];
     }
+    mean = mean2;
+    rstd = rstd2;
   }
   if (P.ws_parts == nullptr) return;
   float* out = P.ws_parts + (int64_t)blockIdx.x * 2 * P.cols;
-  if constexpr (kRows > 1) {
-    constexpr int C = TPR * NV * N;
-    for (int r = 0; r < kRows; ++r) {
-      if (r) __syncthreads();
-      if (sub == r) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    if constexpr (kSets > 1) {
+      const int set = TPR < 64 ? wave : sub;
+      if constexpr (TPR < 64) {
 #pragma unroll
-          for (int j = 0; j < N; ++j) {
-            const int c = (t + i * TPR) * N + j;
-            sums[c] = r ? sums[c] + aw[i][j] : aw[i][j];
-            sums[C + c] = r ? sums[C + c] + ab[i][j] : ab[i][j];
-          }
-      }
-    }
-    __syncthreads();
-    for (int c = threadIdx.x; c < P.cols; c += 256) {
-      out[c] = sums[c];
-      out[P.cols + c] = sums[C + c];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int64_t col = (int64_t)(t + i * TPR) * N;
-#pragma unroll
-      for (int j = 0; j < N; j += 4) {
-        const f32x4 a = {aw[i][j], aw[i][j + 1], aw[i][j + 2], aw[i][j + 3]};
-        const f32x4 c = {ab[i][j], ab[i][j + 1], ab[i][j + 2], ab[i][j + 3]};
-        if (col + j < P.cols) {
-          store16<float>(out, col + j, P.cols, a);
-          store16<float>(out + P.cols, col + j, P.cols, c);
+        for (int j = 0; j < N; ++j) {
+          aw[i][j] = sum_subgroups<TPR>(aw[i][j]);
+          ab[i][j] = sum_subgroups<TPR>(ab[i][j]);
         }
       }
+      if (i) __syncthreads();
+      if (TPR >= 64 || (threadIdx.x & 63) < TPR) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          sums[set][t * N + j] = aw[i][j];
+          sums[set][(TPR + t) * N + j] = ab[i][j];
+        }
+      }
+      __syncthreads();
+      for (int c = threadIdx.x; c < 2 * TPR * N; c += kBwdThreads) {
+        float total = 0.0f;
+        for (int k = 0; k < kSets; ++k) total += sums[k][c];
+        const int which = c / (TPR * N), vec = c % (TPR * N) / N, j = c % N;
+        const Span<T> at(vec + i * TPR, cols);
+        if (j >= at.skip) out[which * P.cols + at.at + j] = total;
+      }
+    } else {
+      const Span<T> at(t + i * TPR, cols);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (j >= at.skip) {
+          out[at.at + j] = aw[i][j];
+          out[P.cols + at.at + j] = ab[i][j];
+        }
     }
   }
 }
@@ -247,6 +331,19 @@ __global__ void __launch_bounds__(1024) k_ln_param_sums(const LnParams P) {
 // Forward: (1) every chunk's mean and sum of squared differences from it, (2) each chunk's workgroup merges the row's
 // chunks and writes its part.  x is read twice, the second time mostly from the caches.
 constexpr int kLongThreads = 256, kLongVecs = 4;
+
+// parameters of columns col ..., as far as they lie inside the row
+template <typename T>
+__device__ __forceinline__ void load_params_part(const void* p, int dtype, int64_t col, int64_t cols, float missing,
+                                                 float (&out)[Elem<T>::kN]) {
+  constexpr int N = Elem<T>::kN;
+  if (p != nullptr && col + N <= cols) {
+    load_params<T>(p, dtype, col, missing, out);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) out[j] = p != nullptr && col + j < cols ? load_as_float(p, dtype, col + j) : missing;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kLongThreads) k_ln_long_stats(const LnParams P) {
@@ -315,8 +412,8 @@ __global__ void __launch_bounds__(kLongThreads) k_ln_long_apply(const LnParams P
   for (int64_t col = c0 + (int64_t)threadIdx.x * N; col < c1; col += kLongThreads * N) {
     const auto v = load16<T>(x, col, c1, (T)0.0f);
     float w[N], b[N];
-    load_params<T>(P.w, P.param_dtype, col, P.cols, 1.0f, w);
-    load_params<T>(P.b, P.param_dtype, col, P.cols, 0.0f, b);
+    load_params_part<T>(P.w, P.param_dtype, col, P.cols, 1.0f, w);
+    load_params_part<T>(P.b, P.param_dtype, col, P.cols, 0.0f, b);
     typename Elem<T>::Vec o;
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] = (T)__builtin_fmaf(((float)v[j] - mean) * rstd, w[j], b[j]);
@@ -339,7 +436,7 @@ __global__ void __launch_bounds__(kLongThreads) k_ln_long_bwd_sums(const LnParam
   for (int64_t col = c0 + (int64_t)threadIdx.x * N; col < c1; col += kLongThreads * N) {
     const auto v = load16<T>(x, col, c1, (T)0.0f), u = load16<T>(dy, col, c1, (T)0.0f);
     float w[N];
-    load_params<T>(P.w, P.param_dtype, col, P.cols, 1.0f, w);
+    load_params_part<T>(P.w, P.param_dtype, col, P.cols, 1.0f, w);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const float g = (float)u[j] * w[j];
@@ -363,7 +460,7 @@ __global__ void __launch_bounds__(kLongThreads) k_ln_long_bwd_apply(const LnPara
   const int64_t col = ((int64_t)blockIdx.x * kLongThreads + threadIdx.x) * N;
   const bool inside = col < P.cols;
   float w[N], aw[N], ab[N];
-  load_params<T>(P.w, P.param_dtype, inside ? col : 0, P.cols, 1.0f, w);
+  load_params_part<T>(P.w, P.param_dtype, inside ? col : 0, P.cols, 1.0f, w);
 #pragma unroll
   for (int j = 0; j < N; ++j) aw[j] = ab[j] = 0.0f;
   for (int64_t row = blockIdx.y; row < P.rows; row += gridDim.y) {
@@ -412,8 +509,9 @@ LnPlan ln_plan(int64_t rows, int64_t cols, int dtype, bool backward) {
   const int n = 16 / dtype_bytes(dtype);
   const int64_t vecs = ceil_div(cols, n);
   struct Shape { int tpr, nv; };
-  static constexpr Shape kFwd[] = {{16, 2}, {64, 1}, {64, 2}, {64, 4}, {64, 8}, {256, 4}, {256, 8}, {1024, 4}, {1024, 8}};
-  static constexpr Shape kBwd[] = {{16, 2}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {512, 4}};
+  static constexpr Shape kFwd[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {512, 4}, {1024, 4},
+                                   {1024, 8}};
+  static constexpr Shape kBwd[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {128, 2}, {256, 2}, {512, 2}, {1024, 2}};
   const Shape* shapes = backward ? kBwd : kFwd;
   const int count = backward ? (int)(sizeof(kBwd) / sizeof(Shape)) : (int)(sizeof(kFwd) / sizeof(Shape));
   for (int i = 0; i < count; ++i)
@@ -423,8 +521,8 @@ LnPlan ln_plan(int64_t rows, int64_t cols, int dtype, bool backward) {
       break;
     }
   if (p.tpr) {
-    const int per = p.tpr <= 64 ? 256 / p.tpr : 1;
-    p.grid = (int)std::min<int64_t>(ceil_div(rows, per), 1024);
+    const int64_t groups = ceil_div(rows, kBwdThreads / p.tpr);
+    p.grid = (int)ceil_div(groups, ceil_div(groups, kBwdBlocks));  // (every workgroup as many rows)
     p.ws_parts = backward ? (int64_t)p.grid * 2 * cols : 0;
     return p;
   }
@@ -470,8 +568,8 @@ int launch_fwd(const LnPlan& p, const LnParams& P, hipStream_t st) {
   const dim3 grid((unsigned)ceil_div(P.rows, per));
 #define UR_LN(TPR, NV) \
   if (p.tpr == TPR && p.nv == NV) k_ln_fwd<T, TPR, NV><<<grid, TPR <= 64 ? 256 : TPR, 0, st>>>(P);
-  UR_LN(16, 2) UR_LN(64, 1) UR_LN(64, 2) UR_LN(64, 4) UR_LN(64, 8) UR_LN(256, 4) UR_LN(256, 8) UR_LN(1024, 4)
-  UR_LN(1024, 8)
+  UR_LN(8, 1) UR_LN(16, 1) UR_LN(32, 1) UR_LN(64, 1) UR_LN(64, 2) UR_LN(64, 4) UR_LN(256, 2) UR_LN(256, 4) UR_LN(512, 4)
+  UR_LN(1024, 4) UR_LN(1024, 8)
 #undef UR_LN
   return launch_status("ur_layer_norm_forward");
 }
@@ -494,8 +592,8 @@ int launch_bwd(const LnPlan& p, const LnParams& P, hipStream_t st) {
   } else {
     const dim3 grid(p.grid);
 #define UR_LN(TPR, NV) \
-  if (p.tpr == TPR && p.nv == NV) k_ln_bwd<T, TPR, NV><<<grid, TPR <= 64 ? 256 : TPR, 0, st>>>(P);
-    UR_LN(16, 2) UR_LN(64, 1) UR_LN(64, 2) UR_LN(64, 4) UR_LN(256, 2) UR_LN(256, 4) UR_LN(512, 4)
+  if (p.tpr == TPR && p.nv == NV) k_ln_bwd<T, TPR, NV><<<grid, kBwdThreads, 0, st>>>(P);
+    UR_LN(8, 1) UR_LN(16, 1) UR_LN(32, 1) UR_LN(64, 1) UR_LN(64, 2) UR_LN(128, 2) UR_LN(256, 2) UR_LN(512, 2) UR_LN(1024, 2)
 #undef UR_LN
   }
   if (P.ws_parts) k_ln_param_sums<<<dim3((unsigned)ceil_div(2 * P.cols, 32)), 1024, 0, st>>>(P);
