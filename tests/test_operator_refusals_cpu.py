@@ -58,9 +58,9 @@ def test_layer_norm_entry_point_checks():
     assert "eps" in refused(*fwd(eps=-1.0))[1] and "eps" in refused(*fwd(eps=float("nan")))[1]
     assert "together" in refused(*fwd(mean=FAKE))[1]
     assert refused(*fwd(D=1 << 20, stride=1 << 20))[0] == -4          # long rows need a workspace
-    n = native.lib().ur_layer_norm_workspace_bytes(4, 8, 0, 1)
+    n = native.lib().ur_layer_norm_workspace_bytes(1000, 8, 0, 1)
     bwd = lambda dy=FAKE, gs=8, x=FAKE, mean=FAKE, rstd=FAKE, gx=FAKE, gw=FAKE, gb=FAKE, ws=FAKE, n=n: (  # noqa: E731
-        "ur_layer_norm_backward", dy, gs, x, 8, None, mean, rstd, 0, 0, 4, 8, gx, gw, gb, ws, n, None)
+        "ur_layer_norm_backward", dy, gs, x, 8, None, mean, rstd, 0, 0, 1000, 8, gx, gw, gb, ws, n, None)
     for k in ("dy", "x", "mean", "rstd"):
         assert refused(*bwd(**{k: None}))[0] == -1
     assert "no gradient" in refused(*bwd(gx=None, gw=None, gb=None))[1]
@@ -76,7 +76,7 @@ def test_layer_norm_workspace_sizes():
         assert size(5, 64, dt, 0) == 0                                 # rows that fit registers: nothing kept
         for M, D in ((1, 1), (7, 33), (100000, 64), (3, 1 << 20), (1, (1 << 31) - 1)):
             n = size(M, D, dt, 1)
-            assert n >= 2 * D * 4 and n % 4 == 0                        # at least one row of partial sums
+            assert n >= (2 * D * 4 if M > 128 else 0) and n % 4 == 0    # rows of partial sums, where several workgroups sum
             assert size(M, D, dt, 0) <= n
 
 

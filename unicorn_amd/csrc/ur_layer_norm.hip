@@ -32,7 +32,7 @@ struct LnParams {
   float* ws;      // partial results of this call
   int64_t chunk;  // long rows: elements of a row one workgroup takes
   int chunks;
-  int parts;      // backward: rows of partial weight sums in `ws_parts`
+  int parts;      // backward: workgroups that sum the parameters' gradients (0: not wanted), each with a row of `ws_parts`
   float* ws_parts;
   void* dw;
   void* db;
@@ -156,6 +156,16 @@ __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR) k_ln_fwd(const LnParams
 // every time.  Large workgroups, one for each CU, because every one of them leaves 2 D floats behind.
 constexpr int kBwdThreads = 1024, kBwdBlocks = 256;
 
+// a workgroup's sum of one column (which: 0 weight, 1 bias): to its partial row, or, from the only workgroup, to the result
+__device__ __forceinline__ void put_sum(const LnParams& P, int part, int which, int64_t col, float v) {
+  if (P.parts > 1) {
+    P.ws_parts[((int64_t)part * 2 + which) * P.cols + col] = v;
+  } else {
+    void* out = which ? P.db : P.dw;
+    if (out) store_from_float(out, P.param_dtype, col, v);
+  }
+}
+
 // adds up what lanes TPR, 2 TPR, ... apart hold
 template <int TPR>
 __device__ __forceinline__ float sum_subgroups(float v) {
@@ -265,8 +275,7 @@ __global__ void __launch_bounds__(kBwdThreads) k_ln_bwd(const LnParams P) {
     mean = mean2;
     rstd = rstd2;
   }
-  if (P.ws_parts == nullptr) return;
-  float* out = P.ws_parts + (int64_t)blockIdx.x * 2 * P.cols;
+  if (P.parts == 0) return;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     if constexpr (kSets > 1) {
@@ -292,15 +301,15 @@ __global__ void __launch_bounds__(kBwdThreads) k_ln_bwd(const LnParams P) {
         for (int k = 0; k < kSets; ++k) total += sums[k][c];
         const int which = c / (TPR * N), vec = c % (TPR * N) / N, j = c % N;
         const Span<T> at(vec + i * TPR, cols);
-        if (j >= at.skip) out[which * P.cols + at.at + j] = total;
+        if (j >= at.skip) put_sum(P, blockIdx.x, which, at.at + j, total);
       }
     } else {
       const Span<T> at(t + i * TPR, cols);
 #pragma unroll
       for (int j = 0; j < N; ++j)
         if (j >= at.skip) {
-          out[at.at + j] = aw[i][j];
-          out[P.cols + at.at + j] = ab[i][j];
+          put_sum(P, blockIdx.x, 0, at.at + j, aw[i][j]);
+          put_sum(P, blockIdx.x, 1, at.at + j, ab[i][j]);
         }
     }
   }
@@ -463,35 +472,46 @@ __global__ void __launch_bounds__(kLongThreads) k_ln_long_bwd_apply(const LnPara
   load_params_part<T>(P.w, P.param_dtype, inside ? col : 0, P.cols, 1.0f, w);
 #pragma unroll
   for (int j = 0; j < N; ++j) aw[j] = ab[j] = 0.0f;
-  for (int64_t row = blockIdx.y; row < P.rows; row += gridDim.y) {
+  struct Fetched {
+    typename Elem<T>::Vec x, dy;
+    float mean, rstd, s0, s1;
+  };
+  const int64_t at = inside ? col : 0;  // (idle threads read along: all lanes take part in the sums)
+  const auto fetch = [&](int64_t row) {
+    Fetched f;
+    f.x = load16<T>(static_cast<const T*>(P.x) + row * P.x_stride, at, P.cols, (T)0.0f);
+    f.dy = load16<T>(static_cast<const T*>(P.dy) + row * P.dy_stride, at, P.cols, (T)0.0f);
+    f.mean = P.mean[row];
+    f.rstd = P.rstd[row];
+    f.s0 = f.s1 = 0.0f;
     const float* st = P.ws + row * P.chunks * 2;
-    float s0 = 0.0f, s1 = 0.0f;
     for (int i = lane; i < P.chunks; i += 64) {
-      s0 += st[2 * i];
-      s1 += st[2 * i + 1];
+      f.s0 += st[2 * i];
+      f.s1 += st[2 * i + 1];
     }
-    const float c1 = reduce_lanes<64, OpSum>(s0) / (float)P.cols, c2 = reduce_lanes<64, OpSum>(s1) / (float)P.cols;
-    if (!inside) continue;
-    const float mean = P.mean[row], rstd = P.rstd[row];
-    const auto v = load16<T>(static_cast<const T*>(P.x) + row * P.x_stride, col, P.cols, (T)0.0f);
-    const auto u = load16<T>(static_cast<const T*>(P.dy) + row * P.dy_stride, col, P.cols, (T)0.0f);
+    return f;
+  };
+  Fetched now = fetch(blockIdx.y);
+  for (int64_t row = blockIdx.y; row < P.rows; row += gridDim.y) {
+    const Fetched next = fetch(min(row + gridDim.y, P.rows - 1));
+    const float c1 = reduce_lanes<64, OpSum>(now.s0) / (float)P.cols, c2 = reduce_lanes<64, OpSum>(now.s1) / (float)P.cols;
     typename Elem<T>::Vec o;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const float h = ((float)v[j] - mean) * rstd, d = (float)u[j];
+      const float h = ((float)now.x[j] - now.mean) * now.rstd, d = (float)now.dy[j];
       aw[j] = __builtin_fmaf(d, h, aw[j]);
       ab[j] += d;
-      o[j] = (T)(rstd * (d * w[j] - c1 - h * c2));
+      o[j] = (T)(now.rstd * (d * w[j] - c1 - h * c2));
     }
-    if (P.y) store16<T>(static_cast<T*>(P.y) + row * P.cols, col, P.cols, o);
+    if (P.y && inside) store16<T>(static_cast<T*>(P.y) + row * P.cols, col, P.cols, o);
+    now = next;
   }
-  if (P.ws_parts == nullptr || !inside) return;
-  float* out = P.ws_parts + (int64_t)blockIdx.y * 2 * P.cols;
+  if (P.parts == 0 || !inside) return;
 #pragma unroll
   for (int j = 0; j < N; ++j)
     if (col + j < P.cols) {
-      out[col + j] = aw[j];
-      out[P.cols + col + j] = ab[j];
+      put_sum(P, blockIdx.y, 0, col + j, aw[j]);
+      put_sum(P, blockIdx.y, 1, col + j, ab[j]);
     }
 }
 
@@ -504,17 +524,21 @@ struct LnPlan {
   int64_t ws_stats, ws_parts;  // floats
 };
 
+// Forward: few rows of more vectors than this are split as well (16 x 65000 bf16: 7.4 against 12.1 us; at 32768 columns or 128
+// rows one workgroup a row is as good or better).
+constexpr int kSplitVecs = 4096, kSplitRows = 64;
 LnPlan ln_plan(int64_t rows, int64_t cols, int dtype, bool backward) {
   LnPlan p{};
   const int n = 16 / dtype_bytes(dtype);
   const int64_t vecs = ceil_div(cols, n);
   struct Shape { int tpr, nv; };
-  static constexpr Shape kFwd[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {512, 4}, {1024, 4},
+  static constexpr Shape kFwd[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {512, 2}, {512, 4}, {1024, 4},
                                    {1024, 8}};
   static constexpr Shape kBwd[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {128, 2}, {256, 2}, {512, 2}, {1024, 2}};
   const Shape* shapes = backward ? kBwd : kFwd;
   const int count = backward ? (int)(sizeof(kBwd) / sizeof(Shape)) : (int)(sizeof(kFwd) / sizeof(Shape));
-  for (int i = 0; i < count; ++i)
+  const bool split = !backward && vecs > kSplitVecs && rows <= kSplitRows;
+  for (int i = 0; i < count && !split; ++i)
     if (vecs <= (int64_t)shapes[i].tpr * shapes[i].nv) {
       p.tpr = shapes[i].tpr;
       p.nv = shapes[i].nv;
@@ -523,16 +547,19 @@ LnPlan ln_plan(int64_t rows, int64_t cols, int dtype, bool backward) {
   if (p.tpr) {
     const int64_t groups = ceil_div(rows, kBwdThreads / p.tpr);
     p.grid = (int)ceil_div(groups, ceil_div(groups, kBwdBlocks));  // (every workgroup as many rows)
-    p.ws_parts = backward ? (int64_t)p.grid * 2 * cols : 0;
+    p.ws_parts = backward && p.grid > 1 ? (int64_t)p.grid * 2 * cols : 0;
     return p;
   }
-  const int64_t step = (int64_t)kLongThreads * kLongVecs * n;
-  p.chunk = ceil_div(ceil_div(cols, 1024), step) * step;  // at most 1024 chunks a row
+  // chunks of at least one vector a thread: about 1024 workgroups in all, at most 1024 for a row
+  const int64_t step = (int64_t)kLongThreads * n;
+  const int64_t per = std::max(ceil_div(cols, 1024), std::min<int64_t>(ceil_div(rows * cols, 1024), kLongVecs * step));
+  p.chunk = ceil_div(per, step) * step;
   p.chunks = (int)ceil_div(cols, p.chunk);
   p.ws_stats = rows * p.chunks * 2;
   const int64_t strips = ceil_div(cols, (int64_t)kLongThreads * n);
-  p.grid = (int)std::min<int64_t>(rows, std::max<int64_t>(1, 2048 / strips));
-  p.ws_parts = backward ? (int64_t)p.grid * 2 * cols : 0;
+  // row ranges: about 1024 workgroups, and at least 8 rows for the 2 D floats a range leaves behind
+  p.grid = (int)std::min<int64_t>(ceil_div(rows, 8), ceil_div(1024, strips));
+  p.ws_parts = backward && p.grid > 1 ? (int64_t)p.grid * 2 * cols : 0;
   return p;
 }
 
@@ -568,7 +595,7 @@ int launch_fwd(const LnPlan& p, const LnParams& P, hipStream_t st) {
   const dim3 grid((unsigned)ceil_div(P.rows, per));
 #define UR_LN(TPR, NV) \
   if (p.tpr == TPR && p.nv == NV) k_ln_fwd<T, TPR, NV><<<grid, TPR <= 64 ? 256 : TPR, 0, st>>>(P);
-  UR_LN(8, 1) UR_LN(16, 1) UR_LN(32, 1) UR_LN(64, 1) UR_LN(64, 2) UR_LN(64, 4) UR_LN(256, 2) UR_LN(256, 4) UR_LN(512, 4)
+  UR_LN(8, 1) UR_LN(16, 1) UR_LN(32, 1) UR_LN(64, 1) UR_LN(64, 2) UR_LN(64, 4) UR_LN(256, 2) UR_LN(512, 2) UR_LN(512, 4)
   UR_LN(1024, 4) UR_LN(1024, 8)
 #undef UR_LN
   return launch_status("ur_layer_norm_forward");
@@ -596,7 +623,7 @@ int launch_bwd(const LnPlan& p, const LnParams& P, hipStream_t st) {
     UR_LN(8, 1) UR_LN(16, 1) UR_LN(32, 1) UR_LN(64, 1) UR_LN(64, 2) UR_LN(128, 2) UR_LN(256, 2) UR_LN(512, 2) UR_LN(1024, 2)
 #undef UR_LN
   }
-  if (P.ws_parts) k_ln_param_sums<<<dim3((unsigned)ceil_div(2 * P.cols, 32)), 1024, 0, st>>>(P);
+  if (P.parts > 1) k_ln_param_sums<<<dim3((unsigned)ceil_div(2 * P.cols, 32)), 1024, 0, st>>>(P);
   return launch_status("ur_layer_norm_backward");
 }
 
@@ -643,14 +670,14 @@ int ur_layer_norm_backward(const void* grad_y, int64_t grad_row_stride, const vo
   if (!grad_x && !grad_weight && !grad_bias) return set_error(UR_ERR_INVALID_ARG, "no gradient asked for");
   const LnPlan p = ln_plan(rows, cols, dtype, true);
   const size_t need = (size_t)(p.ws_stats + p.ws_parts) * 4;
-  if (workspace_bytes < need || !workspace)
+  if (workspace_bytes < need || (need && !workspace))
     return set_error(UR_ERR_WORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, need);
   LnParams P{};
   P.x = x; P.x_stride = x_row_stride; P.dy = grad_y; P.dy_stride = grad_row_stride; P.w = weight;
   P.param_dtype = param_dtype; P.rows = rows; P.cols = cols; P.y = grad_x;
   P.mean = const_cast<float*>(mean); P.rstd = const_cast<float*>(rstd);
   P.ws = static_cast<float*>(workspace); P.chunk = p.chunk; P.chunks = p.chunks;
-  P.parts = p.grid; P.ws_parts = (grad_weight || grad_bias) ? P.ws + p.ws_stats : nullptr;
+  P.parts = (grad_weight || grad_bias) ? p.grid : 0; P.ws_parts = P.ws + p.ws_stats;
   P.dw = grad_weight; P.db = grad_bias;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == UR_F32) return launch_bwd<float>(p, P, st);
