@@ -203,6 +203,14 @@ __device__ __forceinline__ double row_loss(const DistillParams& P, int64_t row, 
   return (double)(float)loss;
 }
 
+// the reduced loss from the sum of the rows' losses and the number of rows that have a teacher; keeps the factor for the
+// backward
+__device__ __forceinline__ void reduced_loss(const DistillParams& P, double sum, double taught) {
+  const double factor = P.reduction == UR_REDUCE_MEAN ? 1.0 / (taught > 0.0 ? taught : 1.0) : 1.0;
+  P.loss[0] = (float)(sum * factor);
+  if (P.stats) P.stats[2 * P.rows] = (float)factor;
+}
+
 // Forward, L lanes a row (a row of few classes), kThreads / L rows a workgroup.
 template <typename T, int L>
 __global__ void __launch_bounds__(kThreads) k_distill_fwd_rows(const DistillParams P) {
@@ -225,10 +233,18 @@ __global__ void __launch_bounds__(kThreads) k_distill_fwd_rows(const DistillPara
     part[1][sub] = mine && taught ? 1.0 : 0.0;
   }
   __syncthreads();
-  if (threadIdx.x >= 2) return;
-  double a = 0.0;
-  for (int r = 0; r < R; ++r) a += part[threadIdx.x][r];
-  P.partial[2 * (int64_t)blockIdx.x + threadIdx.x] = a;
+  if (threadIdx.x) return;
+  double a = 0.0, n = 0.0;
+  for (int r = 0; r < R; ++r) {
+    a += part[0][r];
+    n += part[1][r];
+  }
+  if (P.partials == 1) {
+    reduced_loss(P, a, n);
+  } else {
+    P.partial[2 * (int64_t)blockIdx.x] = a;
+    P.partial[2 * (int64_t)blockIdx.x + 1] = n;
+  }
 }
 
 // a workgroup's maximum and sum, in every thread
@@ -297,7 +313,7 @@ __global__ void __launch_bounds__(64) k_distill_join(const DistillParams P) {
   finish_row<T>(P, row, static_cast<const T*>(P.z) + row * P.stride, m, s);
 }
 
-// sum or mean of the rows' losses, in 64 bits and in a fixed order; keeps the factor for the backward
+// sum or mean of the rows' losses, in 64 bits and in a fixed order
 __global__ void __launch_bounds__(1024) k_distill_reduce(const DistillParams P) {
   __shared__ double part[2][16];
   double a = 0.0, n = 0.0;
@@ -319,9 +335,7 @@ __global__ void __launch_bounds__(1024) k_distill_reduce(const DistillParams P) 
     a += part[0][w];
     n += part[1][w];
   }
-  const double factor = P.reduction == UR_REDUCE_MEAN ? 1.0 / (n > 0.0 ? n : 1.0) : 1.0;
-  P.loss[0] = (float)(a * factor);
-  if (P.stats) P.stats[2 * P.rows] = (float)factor;
+  reduced_loss(P, a, n);
 }
 
 // ---- backward: all of q first, then the teacher's classes are written again with their shares taken off.  A class that
@@ -492,7 +506,7 @@ void launch_fwd(const DistillPlan& p, const DistillParams& P, hipStream_t st) {
     k_distill_split<T><<<dim3(p.splits, rows), kThreads, 0, st>>>(P);
     k_distill_join<T><<<rows, 64, 0, st>>>(P);
   }
-  if (P.reduction != UR_REDUCE_NONE) k_distill_reduce<<<1, 1024, 0, st>>>(P);
+  if (P.reduction != UR_REDUCE_NONE && !(p.lanes && p.partials == 1)) k_distill_reduce<<<1, 1024, 0, st>>>(P);
 }
 
 template <typename T>

@@ -38,19 +38,18 @@ struct RouteParams {
   void* grad;
 };
 
-// ---- order-preserving keys: larger value = larger unsigned number, NaN above everything, 0 = not eligible -----------
+// ---- order-preserving keys: larger value = larger unsigned number, NaN like +inf, 0 = not eligible -------------------
 __device__ __forceinline__ uint64_t order_key(double v) {
-  if (v != v) return ~0ull;
+  if (v != v) v = __builtin_inf();
   const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);  // (-0 -> +0)
   return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
 }
 __device__ __forceinline__ double key_value(uint64_t k) {
-  return __longlong_as_double((long long)((k >> 63) ? (k & 0x7fffffffffffffffull) : ~k));  // (NaN -> NaN)
+  return __longlong_as_double((long long)((k >> 63) ? (k & 0x7fffffffffffffffull) : ~k));
 }
 __device__ __forceinline__ uint32_t order_key(float v) {
-  const uint32_t b = __float_as_uint(v + 0.0f);
-  const uint32_t k = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
-  return v != v ? ~0u : k;
+  const uint32_t b = __float_as_uint(v + 0.0f);  // (not NaN)
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k);
@@ -151,21 +150,29 @@ struct Chosen {
 template <int LPR>
 __device__ __forceinline__ Chosen chosen_share(bool sigmoid, bool renormalize, float l, bool filled, float m, float z) {
   Chosen r{0.0f, 1.0f};
-  const float em = expf(-fabsf(l));  // in (0, 1]: no overflow on either side
-  if (sigmoid) r.comp = l >= 0.0f ? em / (1.0f + em) : 1.0f / (1.0f + em);
-  if (!renormalize) {
-    r.share = !filled ? 0.0f : sigmoid ? (l >= 0.0f ? 1.0f / (1.0f + em) : em / (1.0f + em)) : expf(l - m) / z;
-    if (l != l) r.share = filled ? l : 0.0f;
-    return r;
+  float a, top = 0.0f;
+  if (sigmoid) {
+    const float em = expf(-fabsf(l)), inv = __builtin_amdgcn_rcpf(1.0f + em);  // (em in (0, 1]: no overflow on either side)
+    r.comp = l >= 0.0f ? em * inv : inv;
+    a = l >= 0.0f ? inv : em * inv;
+    // Renormalised, only ratios matter: where all scores of a row are tiny the common factor is left out, so that they share
+    // also below the smallest number.
+    if (renormalize) {
+      top = reduce_lanes<LPR, OpMax>(filled ? __builtin_fminf(l, 0.0f) : -__builtin_inff());
+      if (__any(top < -60.0f)) {
+        if (top < -60.0f) a = expf(__builtin_fminf(l, 0.0f) - top) * inv;
+      }
+    }
+  } else {
+    if (renormalize) top = reduce_lanes<LPR, OpMax>(filled ? l : -__builtin_inff());
+    a = renormalize ? expf(l - top) : expf(l - m) * __builtin_amdgcn_rcpf(z);
   }
-  // only ratios matter: the common factor exp(max) is left out, so scores far below the smallest number still share
-  const float x = sigmoid ? __builtin_fminf(l, 0.0f) : l;
-  const float top = reduce_lanes<LPR, OpMax>(filled ? x : -__builtin_inff());
-  float a = filled ? expf(x - top) : 0.0f;
-  if (sigmoid && filled) a /= 1.0f + em;
-  if (filled && l != l) a = l;
-  const float total = reduce_lanes<LPR, OpSum>(a);
-  r.share = total == 0.0f ? 0.0f : a / total;
+  a = !filled ? 0.0f : l != l ? l : a;
+  r.share = a;
+  if (renormalize) {
+    const float total = reduce_lanes<LPR, OpSum>(a);
+    r.share = total == 0.0f ? 0.0f : a * __builtin_amdgcn_rcpf(total);
+  }
   return r;
 }
 
@@ -191,105 +198,122 @@ __device__ __forceinline__ void row_softmax(const T* __restrict__ row, int E, in
 // largest candidate; the few candidates that reach it (about 10 of 256) go to a list in LDS as (key, index) and each finds its rank
 // by counting the larger ones.
 
-template <int L>
-__device__ __forceinline__ uint32_t max_lanes(uint32_t v) {
-  const auto mx = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
-  if constexpr (L >= 2) v = mx(v, dpp32<kDppXor1>(v));
-  if constexpr (L >= 4) v = mx(v, dpp32<kDppXor2>(v));
-  if constexpr (L >= 8) v = mx(v, dpp32<kDppHalfMirror>(v));
-  if constexpr (L >= 16) v = mx(v, dpp32<kDppMirror>(v));
-  if constexpr (L >= 32) {
-    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    v = mx(r[0], r[1]);
-  }
-  if constexpr (L >= 64) {
-    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    v = mx(r[0], r[1]);
-  }
-  return v;
-}
-
 // how many of the values that a row's other 15 lanes hold (two a lane) are >= v, >= w
 template <int kRor>
-__device__ __forceinline__ void count_ge16(uint32_t v, uint32_t w, int& nv, int& nw) {
+__device__ __forceinline__ void count_ge16(float v, float w, int& nv, int& nw) {
   if constexpr (kRor > 0) {
-    const uint32_t a = dpp32<0x120 + kRor>(v), b = dpp32<0x120 + kRor>(w);
+    const float a = __uint_as_float(dpp32<0x120 + kRor>(__float_as_uint(v)));
+    const float b = __uint_as_float(dpp32<0x120 + kRor>(__float_as_uint(w)));
     nv += (a >= v) + (b >= v);
     nw += (a >= w) + (b >= w);
     count_ge16<kRor - 1>(v, w, nv, nw);
   }
 }
 
-// A lower bound (at least 1) of the (k+1)-th largest key, from the maxima of two sets of keys a lane.  (Two, because groups
-// that were not taken leave lanes empty: with half of 16 lanes left, their 16 sets still bound the 9th largest.)
+// lane i of this lane's row of LPR (i the same in the whole wave)
 template <int LPR>
-__device__ __forceinline__ uint32_t prune_bound(uint32_t v, uint32_t w, int k) {
-  uint32_t bound;
-  if (LPR >= 16 && k + 1 <= 32) {  // 32 sets: lanes 16, 32, 48 apart are put together
-    if constexpr (LPR >= 32) {
-      const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false), q = __builtin_amdgcn_permlane16_swap(w, w, false, false);
-      v = max(r[0], r[1]);
-      w = max(q[0], q[1]);
-    }
-    if constexpr (LPR >= 64) {
-      const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false), q = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-      v = max(r[0], r[1]);
-      w = max(q[0], q[1]);
-    }
+__device__ __forceinline__ float row_lane(float v, int i) {
+  if constexpr (LPR == 64) return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), i));
+  else return __shfl(v, i, LPR);
+}
+
+// maxima over lanes 16 and 32 apart
+template <int LPR>
+__device__ __forceinline__ float max_rows(float v) {
+  if constexpr (LPR >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  if constexpr (LPR >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  return v;
+}
+
+// A lower bound (at least the lowest finite number) of the (k+1)-th largest value, from the maxima of two sets of values a
+// lane.  (Two, because groups that were not taken leave lanes empty: with half of 16 lanes left, their 16 sets still bound
+// the 9th largest.)
+template <int LPR>
+__device__ __forceinline__ float prune_bound(float v, float w, int k) {
+  constexpr float kInf = __builtin_inff();
+  float bound;
+  if (LPR == 16 || (LPR > 16 && k + 1 <= 8)) {  // 32 sets: lanes 16, 32, 48 apart are put together
+    v = max_rows<LPR>(v);
+    w = max_rows<LPR>(w);
     int nv = 1 + (w >= v), nw = 1 + (v >= w);
     count_ge16<15>(v, w, nv, nw);
-    bound = max_lanes<16>(max(nv >= k + 1 ? v : 0u, nw >= k + 1 ? w : 0u));
+    bound = reduce_lanes<16, OpMax>(__builtin_fmaxf(nv >= k + 1 ? v : -kInf, nw >= k + 1 ? w : -kInf));
   } else {
     int nv = 0, nw = 0;
     for (int i = 0; i < LPR; ++i) {
-      const uint32_t a = (uint32_t)__shfl((int)v, i, LPR), b = (uint32_t)__shfl((int)w, i, LPR);
+      const float a = row_lane<LPR>(v, i), b = row_lane<LPR>(w, i);
       nv += (a >= v) + (b >= v);
       nw += (a >= w) + (b >= w);
     }
-    bound = max_lanes<LPR>(max(nv >= k + 1 ? v : 0u, nw >= k + 1 ? w : 0u));
+    bound = reduce_lanes<LPR, OpMax>(__builtin_fmaxf(nv >= k + 1 ? v : -kInf, nw >= k + 1 ? w : -kInf));
   }
-  return bound > 1u ? bound : 1u;
+  return __builtin_fmaxf(bound, -__FLT_MAX__);
 }
 
-// sum of the lanes before this one, inside groups of LPR lanes
+// sum of the lanes before this one, inside groups of LPR lanes (row shifts by DPP, then whole rows of 16)
+template <int kShift>
+__device__ __forceinline__ int add_shifted(int v, int t) {
+  const int up = __builtin_amdgcn_update_dpp(0, v, 0x110 + kShift, 0xf, 0xf, true);
+  return v + (t >= kShift ? up : 0);
+}
 template <int LPR>
 __device__ __forceinline__ int lanes_before(int v, int t) {
-  int incl = v;
+  int incl = add_shifted<1>(v, t & 15);
+  incl = add_shifted<2>(incl, t & 15);
+  incl = add_shifted<4>(incl, t & 15);
+  if constexpr (LPR >= 16) incl = add_shifted<8>(incl, t & 15);
 #pragma unroll
-  for (int o = 1; o < LPR; o <<= 1) {
-    const int up = __shfl_up(incl, o, LPR);
-    if (t >= o) incl += up;
+  for (int o = 16; o < LPR; o <<= 1) {
+    const int up = __shfl(incl, (t & ~(o - 1)) - 1, LPR);  // (the end of the run of lanes before this one's)
+    if (t & o) incl += up;
   }
   return incl - v;
+}
+
+// how many of the other 15 lanes of 16 hold a larger (hi, lo)
+template <int kRor>
+__device__ __forceinline__ int count_larger16(uint32_t hi, uint32_t lo) {
+  if constexpr (kRor == 0) return 0;
+  else {
+    const uint64_t other = ((uint64_t)dpp32<0x120 + kRor>(hi) << 32) | dpp32<0x120 + kRor>(lo);
+    return (other > (((uint64_t)hi << 32) | lo) ? 1 : 0) + count_larger16<kRor - 1>(hi, lo);
+  }
 }
 
 // the hardware's exponential (1 ulp) of the argument rounded to base 2
 __device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
 
+// IPL consecutive logits, as they are stored; -inf behind the row's end
 template <typename T, int IPL>
-__device__ __forceinline__ void load_items(const T* __restrict__ row, int first, int E, float (&l)[IPL]) {
-  struct __attribute__((packed, aligned(sizeof(T)))) Items { T v[IPL]; };
-  if (first + IPL <= E) {
-    const Items it = *reinterpret_cast<const Items*>(row + first);
+struct __attribute__((packed, aligned(sizeof(T)))) Items { T v[IPL]; };
+template <typename T, int IPL>
+__device__ __forceinline__ Items<T, IPL> load_items(const T* __restrict__ row, int first, int E) {
+  if (first + IPL <= E) return *reinterpret_cast<const Items<T, IPL>*>(row + first);
+  Items<T, IPL> it;
 #pragma unroll
-    for (int i = 0; i < IPL; ++i) l[i] = (float)it.v[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < IPL; ++i) l[i] = first + i < E ? (float)row[first + i] : -__builtin_inff();
-  }
+  for (int i = 0; i < IPL; ++i) it.v[i] = first + i < E ? row[first + i] : (T)-__builtin_inff();
+  return it;
 }
 
 template <typename T, int LPR, int IPL>
-__global__ void __launch_bounds__(kThreads) k_route_fwd(const RouteParams P) {
+__global__ void __launch_bounds__(kThreads, 3) k_route_fwd(const RouteParams P) {
   constexpr int R = 64 / LPR, kRow = LPR * IPL;
   constexpr float kInf = __builtin_inff();
   __shared__ int hist[kRow];
-  __shared__ uint64_t lists[kWaves][R * kRow];
+  // a wave's candidates' values, row after row; also one row's keys in 64 bits
+  __shared__ uint64_t store[kWaves][R * kRow / 2 > kRow ? R * kRow / 2 : kRow];
+  __shared__ uint16_t lists[kWaves][R * kRow];  // candidates that reach the bound
   __shared__ uint64_t slot_store[kWaves][R * (LPR + 1)];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / LPR, t = lane % LPR;
-  uint64_t* list = lists[wave] + sub * kRow;
+  float* vals = reinterpret_cast<float*>(store[wave]) + sub * kRow;
+  uint16_t* list = lists[wave] + sub * kRow;
   uint64_t* slots = slot_store[wave] + sub * (LPR + 1);
-  float* vals = reinterpret_cast<float*>(lists[wave]) + sub * kRow;
   const int E = P.cands, first = t * IPL, k = P.top_k, G = P.groups, per = P.per_group;
   for (int e = threadIdx.x; e < E; e += kThreads) hist[e] = 0;
   __syncthreads();
@@ -305,103 +329,150 @@ __global__ void __launch_bounds__(kThreads) k_route_fwd(const RouteParams P) {
 #pragma unroll
   for (int i = 0; i < IPL; ++i) bias[i] = (P.bias && first + i < E) ? P.bias[first + i] : 0.0f;
 
-  const int64_t row_groups = (P.rows + kWaves * R - 1) / (kWaves * R);
-  for (int64_t rg = blockIdx.x; rg < row_groups; rg += gridDim.x) {
-    const int64_t want = (rg * kWaves + wave) * R + sub;
-    const bool mine = want < P.rows;
-    const int64_t row = mine ? want : P.rows - 1;
-    const T* src = static_cast<const T*>(P.logits) + row * P.stride;
-    float l[IPL];
-    load_items<T, IPL>(src, first, E, l);
+  bool odd_bias = false;  // infinities or NaN among the biases
+#pragma unroll
+  for (int i = 0; i < IPL; ++i) odd_bias |= !(fabsf(bias[i]) < kInf);
+  odd_bias = __any(odd_bias);
+
+  const uint32_t last = (uint32_t)P.rows - 1, per_step = kWaves * R, row_groups = last / per_step + 1;
+  const auto row_at = [&](uint32_t row) { return static_cast<const T*>(P.logits) + (uint64_t)row * (uint64_t)P.stride; };
+  uint32_t row = min(blockIdx.x * per_step + wave * R + sub, last);
+  Items<T, IPL> ahead = load_items<T, IPL>(row_at(row), first, E);
+  for (uint32_t rg = blockIdx.x; rg < row_groups; rg += gridDim.x) {
+    const uint32_t want = rg * per_step + wave * R + sub;
+    const bool mine = want <= last;
+    row = min(want, last);
+    const T* src = row_at(row);
+    float c[IPL];  // logits, then what the candidates are compared by; -inf: not eligible
+    float probe = 0.0f;
+#pragma unroll
+    for (int i = 0; i < IPL; ++i) {
+      c[i] = (float)ahead.v[i];
+      probe = __builtin_fmaf(c[i], 0.0f, probe);  // NaN as soon as one logit is not finite
+    }
+    const bool odd = odd_bias || __any(probe != probe);  // (E not a multiple of IPL: the places behind the end are -inf)
+    ahead = load_items<T, IPL>(row_at(min((rg + gridDim.x) * per_step + wave * R + sub, last)), first, E);
 
     // err: bound of two scores' errors.  sigmoid: s (1 - s) (|l| 2^-23.4 + 2^-23) of the exponential, 2^-23 of the
     // reciprocal, 2^-24 of the sum: below 2^-22 each.  softmax, relative to its largest score 1 / z: as much of the
     // exponential and up to 30 roundings of z, below 2^-19 each.
     float m = 0.0f, z = 1.0f, inv_z = 1.0f, err = 0x1p-20f;
     if (need_softmax) {
-      float mf = l[0];
+      float mf = c[0];
 #pragma unroll
-      for (int i = 1; i < IPL; ++i) mf = __builtin_fmaxf(mf, l[i]);
+      for (int i = 1; i < IPL; ++i) mf = __builtin_fmaxf(mf, c[i]);
       mf = reduce_lanes<LPR, OpMax>(mf);
       m = mf == -kInf ? 0.0f : mf;
       float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < IPL; ++i) sum += fast_exp(l[i] - m);
+      for (int i = 0; i < IPL; ++i) sum += fast_exp(c[i] - m);
       z = reduce_lanes<LPR, OpSum>(sum);
       if (z == 0.0f) z = 1.0f;
       inv_z = 1.0f / z;
       err = 0x1p-17f * inv_z;
     }
-    uint32_t key[IPL], gkey[IPL];
+    float a = -kInf, b = -kInf;  // the two largest of this lane's part of its group
+    if (need_scores) {
+      float s[IPL];
+      if (P.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < IPL; ++i) {
-      float c = l[i], s = l[i];
-      if (need_scores) {
-        s = P.sigmoid ? __builtin_amdgcn_rcpf(1.0f + fast_exp(-l[i])) : fast_exp(l[i] - m) * inv_z;
-        if (P.bias) c = s + bias[i];
+        for (int i = 0; i < IPL; ++i) s[i] = __builtin_amdgcn_rcpf(1.0f + fast_exp(-c[i]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < IPL; ++i) s[i] = fast_exp(c[i] - m) * inv_z;
       }
-      const bool ok = l[i] != -kInf && c != -kInf;
-      key[i] = ok ? order_key(c) : 0u;
-      gkey[i] = group_scores ? (ok ? order_key(s) : 0u) : key[i];
+      if (P.bias) {
+#pragma unroll
+        for (int i = 0; i < IPL; ++i) s[i] += bias[i];
+        if (odd) {
+#pragma unroll
+          for (int i = 0; i < IPL; ++i) s[i] = c[i] == -kInf ? -kInf : s[i];
+        }
+#pragma unroll
+        for (int i = 0; i < IPL; ++i) c[i] = s[i];
+      } else {  // the groups' values are of the scores
+#pragma unroll
+        for (int i = 0; i < IPL; ++i) {
+          s[i] = c[i] == -kInf ? -kInf : s[i] != s[i] ? kInf : s[i];
+          if (!whole) vals[first + i] = s[i];
+          const float lo = __builtin_fminf(a, s[i]);
+          a = __builtin_fmaxf(a, s[i]);
+          b = __builtin_fmaxf(b, lo);
+        }
+      }
+    }
+    if (odd) {
+#pragma unroll
+      for (int i = 0; i < IPL; ++i) c[i] = c[i] != c[i] ? kInf : c[i];
     }
 
     bool close = false;  // fp32 cannot tell
+    bool in_group = true;  // (whole groups of lanes) this lane's group is taken
     if (G > 1) {
-      uint32_t a = 0, b = 0;  // the two largest of this lane's group (0: none)
-      int width;              // lanes that hold the same group
-      if (whole) {
-        width = lanes_per;
+      if (!group_scores) {
+        if (whole && !P.top2) {
 #pragma unroll
-        for (int i = 0; i < IPL; ++i) {
-          const uint32_t lo = min(a, gkey[i]);
-          a = max(a, gkey[i]);
-          b = max(b, lo);
+          for (int i = 0; i < IPL; ++i) a = __builtin_fmaxf(a, c[i]);
+        } else if (whole) {
+#pragma unroll
+          for (int i = 0; i < IPL; ++i) {
+            const float lo = __builtin_fminf(a, c[i]);
+            a = __builtin_fmaxf(a, c[i]);
+            b = __builtin_fmaxf(b, lo);
+          }
+        } else {
+          wave_lds_handoff();
+#pragma unroll
+          for (int i = 0; i < IPL; ++i) vals[first + i] = c[i];
         }
-      } else {
-        width = share;
-        wave_lds_handoff();
-#pragma unroll
-        for (int i = 0; i < IPL; ++i) vals[first + i] = __uint_as_float(gkey[i]);
+      }
+      const int width = whole ? lanes_per : share;  // lanes that hold the same group
+      if (!whole) {
         wave_lds_handoff();
         const int g = t / share;
+        a = b = -kInf;
         if (g < G)
           for (int i = t % share; i < per; i += share) {
-            const uint32_t v = __float_as_uint(vals[g * per + i]);
-            const uint32_t lo = min(a, v);
-            a = max(a, v);
-            b = max(b, lo);
+            const float v = vals[g * per + i], lo = __builtin_fminf(a, v);
+            a = __builtin_fmaxf(a, v);
+            b = __builtin_fmaxf(b, lo);
           }
-        wave_lds_handoff();
       }
       for (int o = 1; o < width; o <<= 1) {
-        const uint32_t a2 = (uint32_t)__shfl_xor((int)a, o), b2 = (uint32_t)__shfl_xor((int)b, o);
-        b = max(min(a, a2), max(b, b2));
-        a = max(a, a2);
+        const float a2 = __shfl_xor(a, o), b2 = __shfl_xor(b, o);
+        b = __builtin_fmaxf(__builtin_fminf(a, a2), __builtin_fmaxf(b, b2));
+        a = __builtin_fmaxf(a, a2);
       }
-      const uint32_t g = (P.top2 && a && b) ? order_key(key_value(a) + key_value(b)) : a;
+      const float g = P.top2 && b != -kInf ? a + b : a;
       const int my_group = t / width;
+      // by (value, lower index): a group's rank is the number of groups before it
+      const uint32_t hi = order_key(g), lo = (uint32_t)(kMaxGroups - my_group);
       int rank = 0;
-      uint32_t above = ~0u;  // the smallest of the groups that come before this one
-      for (int o = 0; o < G; ++o) {
-        const uint32_t other = (uint32_t)__shfl((int)g, o * width, LPR);
-        const bool before = other > g || (other == g && o < my_group);
-        rank += before;
-        if (before) above = min(above, other);
+      for (int o = 0; o < G; o += 4) {
+        uint32_t other[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) other[i] = (uint32_t)__shfl((int)hi, min(o + i, G - 1) * width, LPR);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint64_t mine_key = ((uint64_t)hi << 32) | lo;
+          rank += o + i < G && (((uint64_t)other[i] << 32) | (uint32_t)(kMaxGroups - o - i)) > mine_key;
+        }
       }
       const bool taken = my_group < G && rank < P.top_groups;
-      if (need_scores && my_group < G && rank == P.top_groups && g != 0) {
-        const float va = key_value(above), vg = key_value(g);
-        close = va - vg <= 2.0f * err + 0x1p-21f * (fabsf(va) + fabsf(vg));
+      if (need_scores && P.top_groups < G) {  // the last group taken against the first one left
+        const uint64_t at_last = __ballot(my_group < G && rank == P.top_groups - 1) >> (sub * LPR);
+        const float worst = __shfl(g, __builtin_ctzll(at_last), LPR);
+        if (my_group < G && rank == P.top_groups && g != -kInf)
+          close = worst - g <= 2.0f * err + 0x1p-21f * (fabsf(worst) + fabsf(g));
       }
-      const uint64_t kept = (__ballot(taken) >> (sub * LPR));  // bit t: lane t's group is taken
       if (whole) {
-#pragma unroll
-        for (int i = 0; i < IPL; ++i) key[i] = taken ? key[i] : 0u;
+        in_group = taken;
       } else {
+        const uint64_t kept = (__ballot(taken) >> (sub * LPR));  // bit t: lane t's group is taken
         int at = first / per, in = first % per;
 #pragma unroll
         for (int i = 0; i < IPL; ++i) {
-          if (at >= G || !((kept >> (at * share)) & 1)) key[i] = 0u;
+          if (at >= G || !((kept >> (at * share)) & 1)) c[i] = -kInf;
           if (++in == per) {
             in = 0;
             ++at;
@@ -410,45 +481,84 @@ __global__ void __launch_bounds__(kThreads) k_route_fwd(const RouteParams P) {
       }
     }
 
-    // the candidates that can be among the k + 1 largest
-    uint32_t bound = 1u;
+    // the candidates that can be among the k + 1 largest: their places in a list, their values in LDS
+    float bound = -__FLT_MAX__;
     if constexpr (IPL > 1) {
-      uint32_t v = key[0], w = key[IPL / 2];
+      float v = c[0], w = c[IPL / 2];
 #pragma unroll
       for (int i = 1; i < IPL / 2; ++i) {
-        v = max(v, key[i]);
-        w = max(w, key[IPL / 2 + i]);
+        v = __builtin_fmaxf(v, c[i]);
+        w = __builtin_fmaxf(w, c[IPL / 2 + i]);
       }
-      bound = prune_bound<LPR>(v, w, k);
+      bound = prune_bound<LPR>(in_group ? v : -kInf, in_group ? w : -kInf, k);
     }
-    int count = 0;
+    uint32_t reach = 0;
 #pragma unroll
-    for (int i = 0; i < IPL; ++i) count += key[i] >= bound;
-    const int before = lanes_before<LPR>(count, t);
-    const int n = __shfl(before + count, LPR - 1, LPR);
+    for (int i = IPL - 1; i >= 0; --i) reach = 2 * reach + (c[i] >= bound);
+    if (!in_group) reach = 0;
     wave_lds_handoff();
-    list[t] = 0;  // (the first LPR entries are all read below)
-    int pos = before;
 #pragma unroll
-    for (int i = 0; i < IPL; ++i)
-      if (key[i] >= bound) list[pos++] = ((uint64_t)key[i] << 32) | (uint32_t)(kMaxCands - (first + i));
+    for (int i = 0; i < IPL; ++i) vals[first + i] = c[i];
+    int before = lanes_before<LPR>(__popc(reach), t);
+    int n = __shfl(before + __popc(reach), LPR - 1, LPR);
+    if (__any(n > 2 * LPR)) {  // many equal values: of those at the bound the first k + 1 will do
+      uint32_t larger = 0;
+#pragma unroll
+      for (int i = IPL - 1; i >= 0; --i) larger = 2 * larger + (c[i] > bound);
+      larger &= reach;
+      uint32_t equal = reach & ~larger, kept = 0;
+      int left = k + 1 - lanes_before<LPR>(__popc(equal), t);
+      for (; equal && left > 0; --left, equal &= equal - 1) kept |= equal & (0u - equal);
+      reach = larger | kept;
+      before = lanes_before<LPR>(__popc(reach), t);
+      n = __shfl(before + __popc(reach), LPR - 1, LPR);
+    }
+    for (; reach; reach &= reach - 1) list[before++] = (uint16_t)(first + __builtin_ctz(reach));
     for (int j = t; j <= k; j += LPR) slots[j] = 0;
     wave_lds_handoff();
+    const auto entry = [&](int j) {
+      const int e = list[j];
+      return ((uint64_t)order_key(vals[e]) << 32) | (uint32_t)(kMaxCands - e);  // (of equal values the lower index is larger)
+    };
+    uint64_t own = t < n ? entry(t) : 0;
     int n_max = n;
     if constexpr (R > 1) n_max = (int)reduce_lanes<64, OpMax>((float)n);
+    constexpr int kPer = IPL < 8 ? (IPL > 1 ? IPL / 2 : 1) : 4;  // entries a lane that fit over the values
     if (n_max <= LPR) {
-      const uint64_t own = list[t];
       int rank = 0;
-#pragma unroll 4
-      for (int i = 0; i < n_max; ++i) rank += list[i] > own;
+      if constexpr (LPR == 16) {
+        rank = count_larger16<15>((uint32_t)(own >> 32), (uint32_t)own);
+      } else {
+        const float hi = __uint_as_float((uint32_t)(own >> 32)), lo = __uint_as_float((uint32_t)own);
+        for (int i = 0; i < n_max; ++i)
+          rank += (((uint64_t)__float_as_uint(row_lane<LPR>(hi, i)) << 32) | __float_as_uint(row_lane<LPR>(lo, i))) > own;
+      }
       if (own && rank <= k) slots[rank] = own;
+    } else if (n_max <= kPer * LPR) {
+      uint64_t mine_all[kPer];
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) mine_all[q] = t + q * LPR < n ? entry(t + q * LPR) : 0;
+      wave_lds_handoff();
+      uint64_t* entries = store[wave] + sub * (kPer * LPR);
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) entries[t + q * LPR] = mine_all[q];
+      wave_lds_handoff();
+      int rank[kPer] = {};
+#pragma unroll 2
+      for (int i = 0; i < n_max; ++i) {
+        const uint64_t other = entries[i];
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) rank[q] += other > mine_all[q];
+      }
+#pragma unroll
+      for (int q = 0; q < kPer; ++q)
+        if (mine_all[q] && rank[q] <= k) slots[rank[q]] = mine_all[q];
     } else {
-      for (int j0 = 0; j0 < n_max; j0 += LPR) {
-        const int j = j0 + t;
-        const uint64_t own = j < n ? list[j] : ~0ull;
+      for (int j = t; j < n; j += LPR) {
+        own = entry(j);
         int rank = 0;
-        for (int i = 0; i < n_max; ++i) rank += i < n && list[i] > own;
-        if (j < n && rank <= k) slots[rank] = own;
+        for (int i = 0; i < n; ++i) rank += entry(i) > own;
+        if (rank <= k) slots[rank] = own;
       }
     }
     wave_lds_handoff();
@@ -457,8 +567,8 @@ __global__ void __launch_bounds__(kThreads) k_route_fwd(const RouteParams P) {
     int at = got ? kMaxCands - (int)(uint32_t)got : -1;
     if (P.bias && got) {
       const uint64_t next = slots[t + 1];
-      const float c = key_value((uint32_t)(got >> 32)), c2 = key_value((uint32_t)(next >> 32));
-      if (next && c - c2 <= err + 0x1p-22f * (fabsf(c) + fabsf(c2))) {
+      const float v = key_value((uint32_t)(got >> 32)), v2 = key_value((uint32_t)(next >> 32));
+      if (next && v - v2 <= err + 0x1p-22f * (fabsf(v) + fabsf(v2))) {
         const int at2 = kMaxCands - (int)(uint32_t)next;
         close |= !((float)src[at] == (float)src[at2] && P.bias[at] == P.bias[at2]);
       }
@@ -466,8 +576,7 @@ __global__ void __launch_bounds__(kThreads) k_route_fwd(const RouteParams P) {
     uint64_t redo = __ballot(close && mine);
     while (redo) {  // (the whole wave, one row at a time)
       const int r = __builtin_ctzll(redo) / LPR;
-      const int64_t wide_row = (rg * kWaves + wave) * R + r;
-      const int chosen = choose_wide<T>(P, static_cast<const T*>(P.logits) + wide_row * P.stride, lists[wave]);
+      const int chosen = choose_wide<T>(P, row_at(rg * per_step + wave * R + r), store[wave]);
       if (lane < k) slot_store[wave][r * (LPR + 1) + lane] = chosen < 0 ? 0 : (uint64_t)(kMaxCands - chosen);
       wave_lds_handoff();
       if (sub == r && t < k) at = slots[t] ? kMaxCands - (int)(uint32_t)slots[t] : -1;
@@ -476,8 +585,9 @@ __global__ void __launch_bounds__(kThreads) k_route_fwd(const RouteParams P) {
 
     const Chosen ch = chosen_share<LPR>(P.sigmoid, P.renormalize, at >= 0 ? (float)src[at] : 0.0f, at >= 0, m, z);
     if (mine && t < k) {
-      P.weights[row * k + t] = z != z ? z : P.scale * ch.share;  // (a NaN in a softmax is in every score)
-      P.indices[row * k + t] = at;
+      const uint64_t out = (uint64_t)row * (uint32_t)k + t;
+      P.weights[out] = z != z ? z : P.scale * ch.share;  // (a NaN in a softmax is in every score)
+      P.indices[out] = at;
       if (at >= 0) atomicAdd(&hist[at], 1);
     }
   }
@@ -491,8 +601,10 @@ __global__ void __launch_bounds__(1024) k_route_counts(const RouteParams P) {
   __shared__ int acc[32][33];
   const int c = threadIdx.x & 31, grp = threadIdx.x >> 5, e = blockIdx.x * 32 + c;
   int s = 0;
-  if (e < P.cands)
+  if (e < P.cands) {
+#pragma unroll 8
     for (int p = grp; p < P.parts; p += 32) s += P.ws[(int64_t)p * P.cands + e];
+  }
   acc[grp][c] = s;
   __syncthreads();
   if (grp != 0 || e >= P.cands) return;
