@@ -295,7 +295,7 @@ int ur_render_meshes_backward(const float* grad_image, const float* verts, const
  * No counterpart in the reference's native layer (its heads are torch modules; it renders EVERY candidate pose,
  * unicorn.py:295-304, utils/mesh.py:43-71).  Conventions as above, except that tensors may be fp32, fp16 or bf16
  * (UR_F32 / UR_F16 / UR_BF16); sums and statistics are fp32 or wider, a result is rounded to its type once.  Rows may
- * start anywhere (any stride, any alignment of their element type).  Nothing is summed by floating-point atomics: the
+ * start anywhere (any stride, any alignment of their element type); workspaces are 16-byte aligned.  Nothing is summed by floating-point atomics: the
  * same call gives the same bits.
  * ==================================================================================================================== */
 #define UR_F32 0

@@ -190,6 +190,23 @@ def test_ties_go_to_the_lowest_index(cands, k):
                     check_all(logits, k, bias=bias, score=score, **kw)
 
 
+@pytest.mark.parametrize("cands,k", [(16, 4), (33, 10), (64, 6), (64, 20), (100, 12), (256, 8), (256, 15), (300, 16), (512, 31),
+                                     (1024, 8), (1024, 63), (1024, 64)])
+def test_ordered_rows(cands, k):
+    """logits in order of the index: the largest all lie with a few lanes, and little can be ruled out beforehand"""
+    up = torch.linspace(-2, 2, cands, device="cuda")
+    half = torch.cat([up[::2], up[1::2].flip(0)])
+    steps = (up * 6).round() / 6                           # runs of equal values, in order
+    spike = torch.full_like(up, -1.0)
+    spike[cands // 2: cands // 2 + 3] = torch.tensor([0.5, 0.25, 0.5], device="cuda")
+    logits = torch.stack([up, up.flip(0), half, steps, steps.flip(0), spike] * 5)
+    _, bias, _ = make(1, cands, "f32", cands)
+    for b in (None, 0.01 * bias):
+        for kw in ({}, dict(groups=4, top_groups=2, group_score="top2"), dict(groups=4, top_groups=3)):
+            if cands % kw.get("groups", 1) == 0 and k <= kw.get("top_groups", 1) * (cands // kw.get("groups", 1)):
+                check_all(logits, k, bias=b, score="sigmoid", **kw)
+
+
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("cands,k", [(40, 6), (256, 8), (1000, 12)])
 def test_scores_closer_than_float32_can_tell(cands, k, score):

@@ -65,7 +65,7 @@ def test_layer_norm_entry_point_checks():
         assert refused(*bwd(**{k: None}))[0] == -1
     assert "no gradient" in refused(*bwd(gx=None, gw=None, gb=None))[1]
     assert "stride" in refused(*bwd(gs=7))[1]
-    assert refused(*bwd(n=n - 1))[0] == -4 and refused(*bwd(ws=None))[0] == -4
+    assert refused(*bwd(n=n - 1))[0] == -4 and refused(*bwd(ws=None))[0] == -4 and refused(*bwd(ws=FAKE + 8))[0] == -4
     for args in ((0, 8, 0, 0), (4, 0, 0, 0), (4, 8, 3, 0), (1 << 31, 8, 0, 1)):
         assert refused("ur_layer_norm_workspace_bytes", *args)[0] == -1
 
@@ -112,7 +112,7 @@ def test_routing_entry_point_checks():
     for kw in ({"E": 1025, "stride": 1025}, {"E": 128, "stride": 128, "k": 65}, {"E": 130, "stride": 130, "G": 65, "tg": 65},
                {"M": 1 << 31}):
         assert fwd(**kw)[0] == -2, kw
-    assert fwd(M=1000)[0] == -4
+    assert fwd(M=1000)[0] == -4 and fwd(M=1000, ws=FAKE + 4, n=1 << 30)[0] == -4
 
     def bwd(g=FAKE, l=FAKE, dt=0, M=1, E=12, w=FAKE, i=FAKE, k=2, score=0, scale=1.0, out=FAKE):
         return refused("ur_route_backward", g, l, 12, dt, M, E, w, i, k, score, 1, scale, out, None)
@@ -155,6 +155,6 @@ def test_distillation_entry_point_checks():
     for kw in ({"k": 1025}, {"M": 1 << 31}, {"V": 1 << 31, "stride": 1 << 31}):
         assert fwd(**kw)[0] == -2 and bwd(**kw)[0] == -2, kw
     assert fwd(loss=None)[0] == -1 and bwd(g=None)[0] == -1 and bwd(stats=None)[0] == -1 and bwd(out=None)[0] == -1
-    assert fwd(red=2)[0] == -4 and fwd(red=1, ws=FAKE, n=8)[0] == -4
+    assert fwd(red=2)[0] == -4 and fwd(red=1, ws=FAKE, n=8)[0] == -4 and fwd(red=1, ws=FAKE + 8, n=1 << 20)[0] == -4
     for args in ((0, 4, 0, 0), (4, 0, 0, 0), (1 << 31, 4, 0, 0), (4, 4, 3, 0)):
         assert refused("ur_distill_workspace_bytes", *args)[0] == -1

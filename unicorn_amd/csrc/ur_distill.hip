@@ -455,6 +455,7 @@ __global__ void __launch_bounds__(TH) k_distill_bwd(const DistillParams P) {
   __syncthreads();
   const RowGrad r = row_grad(P, row, taught);
   write_q<T, 4>(r, z, out, c0, c1, threadIdx.x, TH);
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the stores have arrived before other waves write the same places
   __syncthreads();
   write_shares<T>(P, r, z, out, cls, share, c0, c1, threadIdx.x, TH);
 }
@@ -566,9 +567,7 @@ int ur_distill_forward(const void* logits, int64_t row_stride, int dtype, int64_
   if (!loss) return set_error(UR_ERR_INVALID_ARG, "null output pointer");
   const DistillPlan plan = distill_plan(rows, cols, dtype, reduction);
   const size_t need = (size_t)plan.ws_bytes;
-  if (workspace_bytes < need || (need && !workspace))
-    return set_error(UR_ERR_WORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, need);
-  if (reinterpret_cast<uintptr_t>(workspace) & 7) return set_error(UR_ERR_WORKSPACE, "workspace must be 8-byte aligned");
+  if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
   DistillParams P{};
   fill_common(P, logits, row_stride, rows, cols, teacher, teacher_dtype, index, index_bytes, top, temperature, reduction);
   P.loss = loss; P.stats = stats;

@@ -648,8 +648,7 @@ int ur_layer_norm_forward(const void* x, int64_t x_row_stride, const void* weigh
   if (!(eps >= 0.0f)) return set_error(UR_ERR_INVALID_ARG, "eps must not be negative");
   const LnPlan p = ln_plan(rows, cols, dtype, false);
   const size_t need = (size_t)(p.ws_stats + p.ws_parts) * 4;
-  if (workspace_bytes < need || (need && !workspace))
-    return set_error(UR_ERR_WORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, need);
+  if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
   LnParams P{};
   P.x = x; P.x_stride = x_row_stride; P.w = weight; P.b = bias; P.param_dtype = param_dtype;
   P.rows = rows; P.cols = cols; P.eps = eps; P.y = y; P.mean = mean; P.rstd = rstd;
@@ -670,8 +669,7 @@ int ur_layer_norm_backward(const void* grad_y, int64_t grad_row_stride, const vo
   if (!grad_x && !grad_weight && !grad_bias) return set_error(UR_ERR_INVALID_ARG, "no gradient asked for");
   const LnPlan p = ln_plan(rows, cols, dtype, true);
   const size_t need = (size_t)(p.ws_stats + p.ws_parts) * 4;
-  if (workspace_bytes < need || (need && !workspace))
-    return set_error(UR_ERR_WORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, need);
+  if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
   LnParams P{};
   P.x = x; P.x_stride = x_row_stride; P.dy = grad_y; P.dy_stride = grad_row_stride; P.w = weight;
   P.param_dtype = param_dtype; P.rows = rows; P.cols = cols; P.y = grad_x;

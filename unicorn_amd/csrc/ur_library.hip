@@ -1,4 +1,4 @@
-// The renderer's translation unit (ur_render.hip as it stands) and, beside its thread-local error buffer, the two
+// The renderer's translation unit (ur_render.hip as it stands) and, beside its thread-local error buffer, the
 // functions through which the other translation units report errors.  -DUR_RENDER_SRC="..." builds the library around
 // another renderer source (timing variants).
 #ifndef UR_RENDER_SRC
@@ -18,5 +18,12 @@ int set_error(int code, const char* fmt, ...) {
 }
 
 int launch_status(const char* what) { return check_launch(what); }
+
+int check_workspace(const void* workspace, size_t bytes, size_t need) {
+  if (need == 0) return UR_OK;
+  if (bytes < need || !workspace) return set_error(UR_ERR_WORKSPACE, "workspace too small: %zu < %zu", workspace ? bytes : 0, need);
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return set_error(UR_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+  return UR_OK;
+}
 
 }  // namespace ur

@@ -746,8 +746,7 @@ int ur_route_forward(const void* logits, int64_t row_stride, int dtype, const fl
     return set_error(UR_ERR_INVALID_ARG, "bad group_score %d", group_score);
   if (!(scale - scale == 0.0f)) return set_error(UR_ERR_INVALID_ARG, "scale must be finite");
   const size_t need = (size_t)ur_route_workspace_bytes(rows, cands);
-  if (workspace_bytes < need || (need && !workspace))
-    return set_error(UR_ERR_WORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, need);
+  if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
   RouteParams P{};
   P.logits = logits; P.stride = row_stride; P.bias = bias; P.rows = rows; P.cands = cands; P.top_k = top_k;
   P.groups = groups; P.per_group = cands / groups; P.top_groups = top_groups;
