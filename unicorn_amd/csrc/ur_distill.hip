@@ -138,33 +138,53 @@ __device__ __forceinline__ bool any_lane(bool v) {
   return ((b >> ((threadIdx.x & 63) / L * L)) & ((1ull << (L & 63)) - 1)) != 0;
 }
 
+// A slot of a row's teacher, and (where z is given) the student's logit of its class.
+struct Slot {
+  int cls;    // -1: empty, -2: a class that there is none of
+  float t, z;
+};
+template <typename T>
+__device__ __forceinline__ Slot slot_at(const DistillParams& P, int64_t row, const T* __restrict__ z, int j) {
+  Slot s{-1, 0.0f, 0.0f};
+  if (j >= P.top) return s;
+  const int64_t c = slot_class(P, row, j);
+  if (c < 0) return s;
+  s.t = load_as_float(P.t, P.t_dtype, row * P.top + j);
+  s.cls = c < P.cols ? (int)c : -2;
+  if (z != nullptr && c < P.cols) s.z = (float)z[c];
+  return s;
+}
+
 // The teacher of a row, by L lanes: maximum and sum of exponentials of its filled slots, and whether there is one; a class
-// outside [0, V) makes the sum NaN.
+// outside [0, V) makes the sum NaN.  `own`: slot threadIdx.x % L, fetched before the row was read (its two dependent
+// loads would stand at the end of every row otherwise).
 struct Teacher {
   float m;
   double s;
   bool any;
 };
-template <int L>
-__device__ __forceinline__ Teacher row_teacher(const DistillParams& P, int64_t row) {
+template <typename T, int L>
+__device__ __forceinline__ Teacher row_teacher(const DistillParams& P, int64_t row, const Slot& own) {
+  constexpr const T* kNoLogits = nullptr;
   const int lane = threadIdx.x % L;
   float m = -__builtin_inff();
   bool any = false, bad = false;
+  Slot at = own;
   for (int j = lane; j < P.top; j += L) {
-    const int64_t c = slot_class(P, row, j);
-    const float t = load_as_float(P.t, P.t_dtype, row * P.top + j);
-    if (c < 0) continue;
-    bad |= c >= P.cols || t != t;
-    any |= t != -__builtin_inff();
-    m = __builtin_fmaxf(m, t);
+    if (j != lane) at = slot_at<T>(P, row, kNoLogits, j);
+    if (at.cls == -1) continue;
+    bad |= at.cls == -2 || at.t != at.t;
+    any |= at.t != -__builtin_inff();
+    m = __builtin_fmaxf(m, at.t);
   }
   m = reduce_lanes<L, OpMax>(m);
   bad = any_lane<L>(bad);
   any = any_lane<L>(any) || bad;
   double s = 0.0;
+  at = own;
   for (int j = lane; j < P.top; j += L) {
-    if (slot_class(P, row, j) < 0) continue;
-    s += (double)exp_slot(load_as_float(P.t, P.t_dtype, row * P.top + j), m, P.scale64);
+    if (j != lane) at = slot_at<T>(P, row, kNoLogits, j);
+    if (at.cls != -1) s += (double)exp_slot(at.t, m, P.scale64);
   }
   s = sum_lanes<L>(s);
   return {m, bad ? __builtin_nan("") : s, any};
@@ -172,24 +192,20 @@ __device__ __forceinline__ Teacher row_teacher(const DistillParams& P, int64_t r
 
 // Loss of a row from its softmax statistics, by L lanes; keeps the statistics and, without a reduction, stores the loss.
 template <typename T, int L>
-__device__ __forceinline__ double row_loss(const DistillParams& P, int64_t row, const T* __restrict__ z, float m, float s, bool store,
-                                           bool& taught) {
+__device__ __forceinline__ double row_loss(const DistillParams& P, int64_t row, const T* __restrict__ z, const Slot& own, float m,
+                                           float s, bool store, bool& taught) {
   const int lane = threadIdx.x % L;
-  const Teacher teacher = row_teacher<L>(P, row);
+  const Teacher teacher = row_teacher<T, L>(P, row, own);
   taught = teacher.any;
   double loss = 0.0;
   const double inv_t = 1.0 / P.temperature, inv_ps = 1.0 / teacher.s;
   const double log_ratio = log((double)s * inv_ps);  // log p - log q = (t - max t) / T - (z - max z) / T + this
+  Slot at = own;
   for (int j = lane; j < P.top; j += L) {
-    const int64_t c = slot_class(P, row, j);
-    if (c < 0 || !teacher.any) continue;
-    if (c >= P.cols) {
-      loss = __builtin_nan("");
-      continue;
-    }
-    const float t = load_as_float(P.t, P.t_dtype, row * P.top + j);
-    const double p = (double)exp_slot(t, teacher.m, P.scale64) * inv_ps;
-    const double d = (((double)t - (double)teacher.m) - ((double)(float)z[c] - (double)m)) * inv_t + log_ratio;
+    if (j != lane) at = slot_at<T>(P, row, z, j);
+    if (at.cls == -1 || !teacher.any) continue;
+    const double p = (double)exp_slot(at.t, teacher.m, P.scale64) * inv_ps;  // (NaN where a class is missing)
+    const double d = (((double)at.t - (double)teacher.m) - ((double)at.z - (double)m)) * inv_t + log_ratio;
     if (p != 0.0) loss += p * d;
   }
   loss = sum_lanes<L>(loss) * P.temperature * P.temperature;
@@ -222,11 +238,12 @@ __global__ void __launch_bounds__(kThreads) k_distill_fwd_rows(const DistillPara
   const int64_t row = mine ? want : P.rows - 1;  // (idle lanes take part in the exchanges)
   const T* z = static_cast<const T*>(P.z) + row * P.stride;
   const float scale = P.scale;
+  const Slot own = slot_at<T>(P, row, z, t);
   float m, s;
   row_part<T, 2>(z, 0, P.cols, t, L, scale, m, s);
   merge_lanes<L>(m, s, scale);
   bool taught;
-  const double loss = row_loss<T, L>(P, row, z, m, s, mine, taught);
+  const double loss = row_loss<T, L>(P, row, z, own, m, s, mine, taught);
   if (P.partial == nullptr) return;
   if (t == 0) {
     part[0][sub] = mine ? loss : 0.0;
@@ -262,9 +279,9 @@ __device__ __forceinline__ void merge_waves(float (&part)[2][W], float& m, float
 }
 
 template <typename T>
-__device__ __forceinline__ void finish_row(const DistillParams& P, int64_t row, const T* z, float m, float s) {
+__device__ __forceinline__ void finish_row(const DistillParams& P, int64_t row, const T* z, const Slot& own, float m, float s) {
   bool taught;
-  const double loss = row_loss<T, 64>(P, row, z, m, s, true, taught);
+  const double loss = row_loss<T, 64>(P, row, z, own, m, s, true, taught);
   if (P.partial && threadIdx.x == 0) {
     P.partial[2 * row] = loss;
     P.partial[2 * row + 1] = taught ? 1.0 : 0.0;
@@ -278,10 +295,12 @@ __global__ void __launch_bounds__(kThreads) k_distill_fwd(const DistillParams P)
   const int64_t row = blockIdx.x;
   const T* z = static_cast<const T*>(P.z) + row * P.stride;
   const float scale = P.scale;
+  Slot own{-1, 0.0f, 0.0f};
+  if (threadIdx.x < 64) own = slot_at<T>(P, row, z, threadIdx.x);
   float m, s;
   row_part<T, 4>(z, 0, P.cols, threadIdx.x, kThreads, scale, m, s);
   merge_waves(part, m, s, scale);
-  if (threadIdx.x < 64) finish_row<T>(P, row, z, m, s);
+  if (threadIdx.x < 64) finish_row<T>(P, row, z, own, m, s);
 }
 
 // Forward, too few rows to fill the chip: a row is split over workgroups, whose maxima and sums a second launch merges.
@@ -304,13 +323,15 @@ template <typename T>
 __global__ void __launch_bounds__(64) k_distill_join(const DistillParams P) {
   const int64_t row = blockIdx.x;
   const float scale = P.scale;
+  const T* z = static_cast<const T*>(P.z) + row * P.stride;
+  const Slot own = slot_at<T>(P, row, z, threadIdx.x);
   float m = -__builtin_inff(), s = 0.0f;
   for (int i = threadIdx.x; i < P.splits; i += 64) {
     const float* in = P.split_stats + 2 * (row * P.splits + i);
     merge(m, s, in[0], in[1], scale);
   }
   merge_lanes<64>(m, s, scale);
-  finish_row<T>(P, row, static_cast<const T*>(P.z) + row * P.stride, m, s);
+  finish_row<T>(P, row, z, own, m, s);
 }
 
 // sum or mean of the rows' losses, in 64 bits and in a fixed order
@@ -342,14 +363,16 @@ __global__ void __launch_bounds__(1024) k_distill_reduce(const DistillParams P) 
 // several slots name gets the sum of their shares, written by the first of them.
 
 // classes and shares of a row's slots, by L lanes; returns 0: no teacher, 1: a teacher, 2: NaN
-template <int L>
+template <typename T, int L>
 __device__ __forceinline__ int row_shares(const DistillParams& P, int64_t row, int* cls, float* share) {
-  const Teacher teacher = row_teacher<L>(P, row);
+  constexpr const T* kNoLogits = nullptr;
+  Slot at = slot_at<T>(P, row, kNoLogits, threadIdx.x % L);
+  const Teacher teacher = row_teacher<T, L>(P, row, at);
   const float inv_s = (float)(1.0 / teacher.s);
   for (int j = threadIdx.x % L; j < P.top; j += L) {
-    const int64_t c = slot_class(P, row, j);
-    cls[j] = (c < 0 || c >= P.cols) ? -1 : (int)c;
-    share[j] = c < 0 ? 0.0f : exp_slot(load_as_float(P.t, P.t_dtype, row * P.top + j), teacher.m, P.scale64) * inv_s;
+    if (j >= L) at = slot_at<T>(P, row, kNoLogits, j);
+    cls[j] = at.cls;
+    share[j] = at.cls == -1 ? 0.0f : exp_slot(at.t, teacher.m, P.scale64) * inv_s;
   }
   return !teacher.any ? 0 : teacher.s != teacher.s ? 2 : 1;
 }
@@ -408,7 +431,7 @@ __device__ __forceinline__ void write_shares(const DistillParams& P, const RowGr
   if (r.zero) return;
   for (int j = t; j < P.top; j += n) {
     const int c = cls[j];
-    if (c < c0 || c >= c1) continue;
+    if (c < c0 || c >= c1 || c < 0) continue;
     float p = 0.0f;
     bool first = true;
     for (int i = 0; i < P.top; ++i)
@@ -432,7 +455,7 @@ __global__ void __launch_bounds__(kThreads) k_distill_bwd_rows(const DistillPara
   const int64_t row = mine ? want : P.rows - 1;
   const T* z = static_cast<const T*>(P.z) + row * P.stride;
   T* out = static_cast<T*>(P.grad) + row * P.cols;
-  const RowGrad r = row_grad(P, row, row_shares<L>(P, row, cls[sub], share[sub]));
+  const RowGrad r = row_grad(P, row, row_shares<T, L>(P, row, cls[sub], share[sub]));
   if (mine) write_q<T, 2>(r, z, out, 0, P.cols, t, L);
   wave_lds_handoff();
   if (mine) write_shares<T>(P, r, z, out, cls[sub], share[sub], 0, P.cols, t, L);
@@ -449,7 +472,7 @@ __global__ void __launch_bounds__(TH) k_distill_bwd(const DistillParams P) {
   const T* z = static_cast<const T*>(P.z) + row * P.stride;
   T* out = static_cast<T*>(P.grad) + row * P.cols;
   if (threadIdx.x < 64) {
-    const int state = row_shares<64>(P, row, cls, share);
+    const int state = row_shares<T, 64>(P, row, cls, share);
     if (threadIdx.x == 0) taught = state;
   }
   __syncthreads();
