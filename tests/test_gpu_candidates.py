@@ -192,3 +192,54 @@ def test_captured_candidate_step():
         torch.cuda.synchronize()
         for a, b in zip(out, eager):
             assert torch.equal(a, b)
+
+
+def _operators(x, w):
+    """every operator of the step, from a leaf"""
+    from unicorn_amd.distillation import distill_top_logits
+    from unicorn_amd.normalization import layer_norm
+    from unicorn_amd.routing import route_candidates
+    index = torch.arange(2, device="cuda").repeat(len(x), 1)
+    return {"layer_norm": lambda: layer_norm(x, w), "route_candidates": lambda: route_candidates(x, 2).weights,
+            "distill_top_logits": lambda: distill_top_logits(x, x.detach()[:, :2].contiguous(), index)}
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "route_candidates", "distill_top_logits"])
+def test_forward_mode_is_refused(name):
+    import torch.autograd.forward_ad as fwd
+    x, w = torch.randn(5, 8, device="cuda"), torch.ones(8, device="cuda")
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            _operators(dual, w)[name]()
+    _operators(x, w)[name]()
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "route_candidates", "distill_top_logits"])
+def test_captured_backward_beside_an_eager_graph_of_the_same_leaf_is_refused(name):
+    """the leaf's accumulator belongs to the default stream as long as the eager graph lives; without that graph, the
+    capture works"""
+    x = torch.randn(5, 8, device="cuda").requires_grad_(True)
+    w = torch.ones(8, device="cuda", requires_grad=True)
+    op = _operators(x, w)[name]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        op().sum().backward()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    eager = op()
+    with pytest.raises(RuntimeError, match="default stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            op().sum().backward()
+    eager.sum().backward()  # (the eager graph is as good as before)
+    want = torch.autograd.grad(op().sum(), x)[0]
+    del eager
+    x.grad = w.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        op().sum().backward()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(x.grad, want)

@@ -10,7 +10,9 @@
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -113,6 +115,27 @@ void* ptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr
 const void* cptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 Tensor or_none(const std::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 
+// The nodes know nothing of forward-mode differentiation: a tangent would be dropped without a word.
+void no_tangent(std::initializer_list<Tensor> inputs) {
+  for (const Tensor& t : inputs)
+    if (t.defined() && t._fw_grad(0).defined())
+      throw std::runtime_error("forward-mode differentiation is not supported by this operator");
+}
+
+// A leaf's gradient accumulator belongs to the stream of the graph that made it and lives as long as that graph.  A captured
+// backward that meets one of the default stream would make the default stream part of the capture, which ends the process.
+void no_accumulator_of_default_stream(const Node& node) {
+  for (const auto& edge : node.next_edges()) {
+    if (!edge.function || !dynamic_cast<const torch::autograd::AccumulateGrad*>(edge.function.get())) continue;
+    const c10::Stream made_on = edge.function->input_metadata(0).stream();
+    if (made_on.device_type() != c10::DeviceType::HIP && made_on.device_type() != c10::DeviceType::CUDA) continue;
+    if (made_on.id() != 0 || c10::hip::getCurrentHIPStream(made_on.device_index()).id() == 0) continue;
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+      throw std::runtime_error("a backward pass is being captured while a graph that was recorded on the default stream from the "
+                               "same leaf is alive: drop that graph (its outputs) before the capture");
+  }
+}
+
 // What a backward returns under create_graph: differentiating it again raises (the kernels are not recorded).
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -185,6 +208,7 @@ struct LayerNormBackward : Node {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(3);
     if (!grads[0].defined()) return out;
+    no_accumulator_of_default_stream(*this);
     const Tensor xs = x.unpack(), ws = weight.unpack();
     std::tie(out[0], out[1], out[2]) =
         layer_norm_backward(grads[0], xs, ws, param_dtype, stats, task_should_compute_output(0), task_should_compute_output(1),
@@ -202,6 +226,7 @@ struct LayerNormBackward : Node {
 
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
   const Tensor w = or_none(weight), b = or_none(bias);
+  no_tangent({x, w, b});
   const bool record = compute_requires_grad(x, w, b);
   auto [y, stats] = layer_norm_forward(x, w, b, eps, record);
   if (record) {
@@ -265,6 +290,7 @@ struct RouteBackward : Node {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(1);
     if (!grads[0].defined()) return out;
+    no_accumulator_of_default_stream(*this);
     out[0] = route_backward(grads[0], logits.unpack(), weights.unpack(shared_from_this()), indices.unpack(), score, renormalize,
                             scale);
     return once(std::move(out));
@@ -281,6 +307,7 @@ struct RouteBackward : Node {
 std::tuple<Tensor, Tensor, Tensor> route(const Tensor& logits, const std::optional<Tensor>& bias, int64_t top_k, int64_t score,
                                          int64_t groups, int64_t top_groups, int64_t group_score, bool renormalize,
                                          double scale) {
+  no_tangent({logits});
   auto out = route_forward(logits, bias, top_k, score, groups, top_groups, group_score, renormalize, scale);
   if (compute_requires_grad(logits)) {
     auto node = std::make_shared<RouteBackward>();
@@ -346,6 +373,7 @@ struct DistillBackward : Node {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(1);
     if (!grads[0].defined()) return out;
+    no_accumulator_of_default_stream(*this);
     const Tensor z = logits.unpack();
     out[0] = distill_backward(grads[0], z, teacher.unpack(), index.unpack(), temperature, reduction, stats);
     return once(std::move(out));
@@ -361,6 +389,7 @@ struct DistillBackward : Node {
 };
 
 Tensor distill(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature, int64_t reduction) {
+  no_tangent({logits});
   const bool record = compute_requires_grad(logits);
   auto [loss, stats] = distill_forward(logits, teacher, index, temperature, reduction, record);
   if (record) {
