@@ -326,3 +326,23 @@ def test_captured_step(rows, cols, k):
         el, eg = run(z2, t2, i2)
         torch.cuda.synchronize()
         assert torch.equal(loss, el) and torch.equal(grad, eg)
+
+
+def test_more_rows_than_a_launch_holds_threads_for():
+    from unicorn_amd.distillation import distill_top_logits
+    g = torch.Generator(device="cuda").manual_seed(4)
+    z = torch.randn(4096, 2, generator=g, device="cuda").half()
+    t = torch.randn(4096, 1, generator=g, device="cuda").half()
+    i = torch.randint(-1, 2, (4096, 1), generator=g, device="cuda", dtype=torch.int32)
+    n = 2 ** 29 // 4096 + 1  # 8 lanes a row: 2^32 threads and some
+    results = []
+    for times in (1, n):
+        x = z.repeat(times, 1).requires_grad_(True)
+        loss = distill_top_logits(x, t.repeat(times, 1), i.repeat(times, 1), reduction="none")
+        results.append((loss.detach(), torch.autograd.grad(loss, x, torch.ones((), device="cuda").expand_as(loss))[0]))
+        mean = distill_top_logits(x.detach(), t.repeat(times, 1), i.repeat(times, 1))
+        # the same rows over again: in 64 bits the mean differs by the roundings of 2^29 additions at most, then one to float32
+        results[-1] += (mean,)
+    (loss, grad, mean), (loss_n, grad_n, mean_n) = results
+    assert bool((loss_n.view(-1, 4096) == loss).all()) and bool((grad_n.view(-1, 8192) == grad.view(1, 8192)).all())
+    assert abs(mean_n.item() - mean.item()) <= 2 ** 29 * 2.0 ** -53 * abs(mean.item()) + 2.0 ** -24 * 2 * abs(mean.item())

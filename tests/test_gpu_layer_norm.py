@@ -314,3 +314,12 @@ def test_module():
     assert len(list(LayerNorm(40, bias=False).parameters())) == 1
     with pytest.raises(ValueError, match="last dimension of 40"):
         ln(torch.randn(6, 41, device="cuda"))
+
+
+def test_more_rows_than_a_launch_holds_threads_for():
+    from unicorn_amd.normalization import layer_norm
+    part = make(4096, 2, torch.float16, torch.float16, seed=3)[0]
+    x = part.repeat(2 ** 29 // 4096 + 1, 1)  # 8 lanes a row: 2^32 threads and some
+    y = layer_norm(x)
+    check(y[:4096], reference(part, None, None, 1e-5)["y"], "y")
+    assert bool((y.view(-1, 8192) == y[:4096].view(1, 8192)).all())

@@ -403,3 +403,31 @@ def test_balance_bias_evens_out_the_choices():
         assert update_balance_bias(bias, counts, 0.005) is bias
         assert torch.equal(bias, before + 0.005 * torch.sign(counts.float().mean() - counts))
     assert float(counts.float().std()) < 0.2 * float(first.std())
+
+
+def test_lowest_numbers_as_biases_under_pairs_of_a_group():
+    """two biases of the lowest number add up to less than float32 holds: still more than a group that has nothing eligible"""
+    low = torch.finfo(torch.float32).min
+    l = torch.randn(6, 12, generator=torch.Generator().manual_seed(1)).cuda()
+    l[:, :3] = -INF
+    l[3:, 9:] = -INF
+    bias = torch.tensor([0.0] * 3 + [low] * 6 + [0.5 * low] * 3, device="cuda")
+    for score in ("softmax", "sigmoid"):
+        for k, top in ((1, 1), (3, 2), (5, 3)):
+            check_all(l, k, bias=bias, score=score, groups=4, top_groups=top, group_score="top2")
+    high = torch.tensor([0.1] * 3 + [-low] * 3 + [-0.75 * low] * 6, device="cuda")
+    for k, top in ((1, 1), (3, 2), (5, 3)):
+        check_all(l, k, bias=high, score="sigmoid", groups=4, top_groups=top, group_score="top2")
+
+
+def test_more_rows_than_a_launch_holds_threads_for():
+    from unicorn_amd.routing import route_candidates
+    part = make(4096, 2, "f16", 5)[0]
+    x = part.repeat(2 ** 29 // 4096 + 1, 1).requires_grad_(True)  # 8 lanes a row: 2^32 threads and some in the backward
+    small = part.clone().requires_grad_(True)
+    grads = []
+    for t in (small, x):
+        r = route_candidates(t, 1, renormalize=False)
+        grads.append(torch.autograd.grad(r.weights, t, torch.ones((), device="cuda").expand_as(r.weights))[0])
+    assert r.counts.sum().item() == len(x)
+    assert bool((grads[1].view(-1, 8192) == grads[0].view(1, 8192)).all())

@@ -24,6 +24,7 @@ struct DistillParams {
   const void* z;
   int64_t stride;
   int64_t rows, cols;
+  int64_t block0;  // the first workgroup of this launch
   const void* t;
   int t_dtype;
   const void* index;
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(kThreads) k_distill_fwd_rows(const DistillPara
   constexpr int R = kThreads / L;
   __shared__ double part[2][R];
   const int t = threadIdx.x % L, sub = threadIdx.x / L;
-  const int64_t want = (int64_t)blockIdx.x * R + sub;
+  const int64_t want = (P.block0 + blockIdx.x) * R + sub;
   const bool mine = want < P.rows;
   const int64_t row = mine ? want : P.rows - 1;  // (idle lanes take part in the exchanges)
   const T* z = static_cast<const T*>(P.z) + row * P.stride;
@@ -259,8 +260,8 @@ __global__ void __launch_bounds__(kThreads) k_distill_fwd_rows(const DistillPara
   if (P.partials == 1) {
     reduced_loss(P, a, n);
   } else {
-    P.partial[2 * (int64_t)blockIdx.x] = a;
-    P.partial[2 * (int64_t)blockIdx.x + 1] = n;
+    P.partial[2 * (P.block0 + blockIdx.x)] = a;
+    P.partial[2 * (P.block0 + blockIdx.x) + 1] = n;
   }
 }
 
@@ -292,7 +293,7 @@ __device__ __forceinline__ void finish_row(const DistillParams& P, int64_t row, 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_distill_fwd(const DistillParams P) {
   __shared__ float part[2][kThreads / 64];
-  const int64_t row = blockIdx.x;
+  const int64_t row = P.block0 + blockIdx.x;
   const T* z = static_cast<const T*>(P.z) + row * P.stride;
   const float scale = P.scale;
   Slot own{-1, 0.0f, 0.0f};
@@ -450,7 +451,7 @@ __global__ void __launch_bounds__(kThreads) k_distill_bwd_rows(const DistillPara
   __shared__ int cls[R][kGroupTop];
   __shared__ float share[R][kGroupTop];
   const int t = threadIdx.x % L, sub = threadIdx.x / L;
-  const int64_t want = (int64_t)blockIdx.x * R + sub;
+  const int64_t want = (P.block0 + blockIdx.x) * R + sub;
   const bool mine = want < P.rows;
   const int64_t row = mine ? want : P.rows - 1;
   const T* z = static_cast<const T*>(P.z) + row * P.stride;
@@ -467,7 +468,7 @@ __global__ void __launch_bounds__(TH) k_distill_bwd(const DistillParams P) {
   __shared__ int cls[kMaxTop];
   __shared__ float share[kMaxTop];
   __shared__ int taught;
-  const int64_t row = P.splits > 1 ? blockIdx.y : blockIdx.x;
+  const int64_t row = P.splits > 1 ? blockIdx.y : P.block0 + blockIdx.x;
   const int64_t c0 = P.splits > 1 ? (int64_t)blockIdx.x * P.chunk : 0, c1 = P.splits > 1 ? min(c0 + P.chunk, P.cols) : P.cols;
   const T* z = static_cast<const T*>(P.z) + row * P.stride;
   T* out = static_cast<T*>(P.grad) + row * P.cols;
@@ -521,29 +522,39 @@ DistillPlan distill_plan(int64_t rows, int64_t cols, int dtype, int reduction) {
 
 template <typename T>
 void launch_fwd(const DistillPlan& p, const DistillParams& P, hipStream_t st) {
-  const unsigned rows = (unsigned)P.rows, groups = (unsigned)p.partials;
-  if (p.lanes == 8) k_distill_fwd_rows<T, 8><<<groups, kThreads, 0, st>>>(P);
-  else if (p.lanes == 16) k_distill_fwd_rows<T, 16><<<groups, kThreads, 0, st>>>(P);
-  else if (p.lanes == 64) k_distill_fwd_rows<T, 64><<<groups, kThreads, 0, st>>>(P);
-  else if (p.splits == 1) k_distill_fwd<T><<<rows, kThreads, 0, st>>>(P);
-  else {
-    k_distill_split<T><<<dim3(p.splits, rows), kThreads, 0, st>>>(P);
-    k_distill_join<T><<<rows, 64, 0, st>>>(P);
+  if (p.splits > 1) {
+    k_distill_split<T><<<dim3(p.splits, (unsigned)P.rows), kThreads, 0, st>>>(P);
+    k_distill_join<T><<<(unsigned)P.rows, 64, 0, st>>>(P);
+  } else {
+    in_pieces(p.lanes ? p.partials : P.rows, kThreads, [&](int64_t first, unsigned grid) {
+      DistillParams Q = P;
+      Q.block0 = first;
+      if (p.lanes == 8) k_distill_fwd_rows<T, 8><<<grid, kThreads, 0, st>>>(Q);
+      else if (p.lanes == 16) k_distill_fwd_rows<T, 16><<<grid, kThreads, 0, st>>>(Q);
+      else if (p.lanes == 64) k_distill_fwd_rows<T, 64><<<grid, kThreads, 0, st>>>(Q);
+      else k_distill_fwd<T><<<grid, kThreads, 0, st>>>(Q);
+    });
   }
   if (P.reduction != UR_REDUCE_NONE && !(p.lanes && p.partials == 1)) k_distill_reduce<<<1, 1024, 0, st>>>(P);
 }
 
 template <typename T>
 void launch_bwd(const DistillPlan& p, const DistillParams& P, hipStream_t st) {
-  const unsigned rows = (unsigned)P.rows;
+  if (p.splits > 1) {
+    k_distill_bwd<T, 256><<<dim3(p.splits, (unsigned)P.rows), 256, 0, st>>>(P);
+    return;
+  }
   const int lanes = P.top <= kGroupTop ? p.lanes : 0;
-  if (lanes == 8) k_distill_bwd_rows<T, 8><<<(unsigned)ceil_div(P.rows, 32), kThreads, 0, st>>>(P);
-  else if (lanes == 16) k_distill_bwd_rows<T, 16><<<(unsigned)ceil_div(P.rows, 16), kThreads, 0, st>>>(P);
-  else if (lanes == 64) k_distill_bwd_rows<T, 64><<<(unsigned)ceil_div(P.rows, 4), kThreads, 0, st>>>(P);
-  else if (p.splits > 1) k_distill_bwd<T, 256><<<dim3(p.splits, rows), 256, 0, st>>>(P);
-  else if (p.bwd_threads == 256) k_distill_bwd<T, 256><<<rows, 256, 0, st>>>(P);
-  else if (p.bwd_threads == 512) k_distill_bwd<T, 512><<<rows, 512, 0, st>>>(P);
-  else k_distill_bwd<T, 1024><<<rows, 1024, 0, st>>>(P);
+  in_pieces(lanes ? ceil_div(P.rows, kThreads / lanes) : P.rows, lanes ? kThreads : p.bwd_threads, [&](int64_t first, unsigned grid) {
+    DistillParams Q = P;
+    Q.block0 = first;
+    if (lanes == 8) k_distill_bwd_rows<T, 8><<<grid, kThreads, 0, st>>>(Q);
+    else if (lanes == 16) k_distill_bwd_rows<T, 16><<<grid, kThreads, 0, st>>>(Q);
+    else if (lanes == 64) k_distill_bwd_rows<T, 64><<<grid, kThreads, 0, st>>>(Q);
+    else if (p.bwd_threads == 256) k_distill_bwd<T, 256><<<grid, 256, 0, st>>>(Q);
+    else if (p.bwd_threads == 512) k_distill_bwd<T, 512><<<grid, 512, 0, st>>>(Q);
+    else k_distill_bwd<T, 1024><<<grid, 1024, 0, st>>>(Q);
+  });
 }
 
 int check_common(const void* logits, int64_t stride, int dtype, int64_t rows, int64_t cols, const void* teacher,

@@ -25,6 +25,7 @@ struct LnParams {
   const void* b;
   int param_dtype;
   int64_t rows, cols;
+  int64_t block0;  // the first workgroup of this launch
   float eps;
   void* y;  // forward: y; backward: dx
   float* mean;
@@ -102,7 +103,7 @@ __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR) k_ln_fwd(const LnParams
   constexpr int N = Elem<T>::kN, kRows = TPR <= 64 ? 256 / TPR : 1;
   __shared__ float part[2][TPR <= 64 ? 1 : TPR / 64];
   const int t = threadIdx.x % TPR, cols = (int)P.cols;
-  const int64_t want = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
+  const int64_t want = (P.block0 + blockIdx.x) * kRows + threadIdx.x / TPR;
   const bool mine = want < P.rows;
   const int64_t row = mine ? want : P.rows - 1;  // (idle lanes take part in the lane exchanges)
   const T* x = static_cast<const T*>(P.x) + row * P.x_stride;
@@ -678,12 +679,15 @@ int launch_fwd(const LnPlan& p, const LnParams& P, hipStream_t st) {
     return launch_status("ur_layer_norm_forward");
   }
   const int per = p.tpr <= 64 ? 256 / p.tpr : 1;
-  const dim3 grid((unsigned)ceil_div(P.rows, per));
+  in_pieces(ceil_div(P.rows, per), p.tpr <= 64 ? 256 : p.tpr, [&](int64_t first, unsigned grid) {
+    LnParams Q = P;
+    Q.block0 = first;
 #define UR_LN(TPR, NV) \
-  if (p.tpr == TPR && p.nv == NV) k_ln_fwd<T, TPR, NV><<<grid, TPR <= 64 ? 256 : TPR, 0, st>>>(P);
-  UR_LN(8, 1) UR_LN(16, 1) UR_LN(32, 1) UR_LN(64, 1) UR_LN(64, 2) UR_LN(64, 4) UR_LN(256, 2) UR_LN(512, 2) UR_LN(512, 4)
-  UR_LN(1024, 4) UR_LN(1024, 8)
+  if (p.tpr == TPR && p.nv == NV) k_ln_fwd<T, TPR, NV><<<grid, TPR <= 64 ? 256 : TPR, 0, st>>>(Q);
+    UR_LN(8, 1) UR_LN(16, 1) UR_LN(32, 1) UR_LN(64, 1) UR_LN(64, 2) UR_LN(64, 4) UR_LN(256, 2) UR_LN(512, 2) UR_LN(512, 4)
+    UR_LN(1024, 4) UR_LN(1024, 8)
 #undef UR_LN
+  });
   return launch_status("ur_layer_norm_forward");
 }
 

@@ -26,6 +26,7 @@ struct RouteParams {
   int64_t stride;
   const float* bias;
   int64_t rows;
+  int64_t block0;  // the first workgroup of this launch
   int cands, top_k, groups, per_group, top_groups;
   bool sigmoid, top2, renormalize;
   float scale;
@@ -443,7 +444,8 @@ __global__ void __launch_bounds__(kThreads, 3) k_route_fwd(const RouteParams P) 
         b = __builtin_fmaxf(__builtin_fminf(a, a2), __builtin_fmaxf(b, b2));
         a = __builtin_fmaxf(a, a2);
       }
-      const float g = P.top2 && b != -kInf ? a + b : a;
+      // (two biases of the lowest number stay above a group that nothing is eligible of)
+      const float g = P.top2 && b != -kInf ? __builtin_fmaxf(a + b, -__FLT_MAX__) : a;
       const int my_group = t / width;
       // by (value, lower index): a group's rank is the number of groups before it
       const uint32_t hi = order_key(g), lo = (uint32_t)(kMaxGroups - my_group);
@@ -463,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_route_fwd(const RouteParams P) 
         const uint64_t at_last = __ballot(my_group < G && rank == P.top_groups - 1) >> (sub * LPR);
         const float worst = __shfl(g, __builtin_ctzll(at_last), LPR);
         if (my_group < G && rank == P.top_groups && g != -kInf)
-          close = worst - g <= 2.0f * err + 0x1p-21f * (fabsf(worst) + fabsf(g));
+          close = !(worst - g > 2.0f * err + 0x1p-21f * (fabsf(worst) + fabsf(g)));  // (inf - inf: cannot tell)
       }
       if (whole) {
         in_group = taken;
@@ -625,7 +627,7 @@ __global__ void __launch_bounds__(kThreads) k_route_bwd(const RouteParams P) {
   __shared__ __align__(16) float rows[kWaves][R * kRow];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / LPR, t = lane % LPR;
   float* acc = rows[wave] + sub * kRow;
-  const int64_t want = ((int64_t)blockIdx.x * kWaves + wave) * R + sub;
+  const int64_t want = ((P.block0 + blockIdx.x) * kWaves + wave) * R + sub;
   const bool mine = want < P.rows;
   const int64_t row = mine ? want : P.rows - 1;
   const T* l = static_cast<const T*>(P.logits) + row * P.stride;
@@ -713,11 +715,14 @@ void launch_fwd(const RouteParams& P, RouteShape s, hipStream_t st) {
 
 template <typename T>
 void launch_bwd(const RouteParams& P, int lpr, hipStream_t st) {
-  const unsigned grid = (unsigned)ceil_div(P.rows, kWaves * (64 / lpr));
-  if (lpr == 8) k_route_bwd<T, 8><<<grid, kThreads, 0, st>>>(P);
-  else if (lpr == 16) k_route_bwd<T, 16><<<grid, kThreads, 0, st>>>(P);
-  else if (lpr == 32) k_route_bwd<T, 32><<<grid, kThreads, 0, st>>>(P);
-  else k_route_bwd<T, 64><<<grid, kThreads, 0, st>>>(P);
+  in_pieces(ceil_div(P.rows, kWaves * (64 / lpr)), kThreads, [&](int64_t first, unsigned grid) {
+    RouteParams Q = P;
+    Q.block0 = first;
+    if (lpr == 8) k_route_bwd<T, 8><<<grid, kThreads, 0, st>>>(Q);
+    else if (lpr == 16) k_route_bwd<T, 16><<<grid, kThreads, 0, st>>>(Q);
+    else if (lpr == 32) k_route_bwd<T, 32><<<grid, kThreads, 0, st>>>(Q);
+    else k_route_bwd<T, 64><<<grid, kThreads, 0, st>>>(Q);
+  });
 }
 
 }  // namespace

@@ -129,6 +129,14 @@ __device__ __forceinline__ void wave_lds_handoff() {
 }
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// A launch holds less than 2^32 threads (2^29 rows of 8 lanes are more): larger grids go out in pieces, launch(first
+// workgroup, workgroups).
+template <typename F>
+void in_pieces(int64_t blocks, int threads, const F& launch) {
+  const int64_t most = 0xffffffffll / threads;
+  for (int64_t b = 0; b < blocks; b += most) launch(b, (unsigned)(blocks - b < most ? blocks - b : most));
+}
 inline bool known_dtype(int d) { return d == UR_F32 || d == UR_F16 || d == UR_BF16; }
 inline int dtype_bytes(int d) { return d == UR_F32 ? 4 : 2; }
 
