@@ -19,7 +19,11 @@ namespace {
 constexpr int kMaxCands = 1024, kMaxTop = 64, kMaxGroups = 64;
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 typedef float f32x4_lds __attribute__((ext_vector_type(4)));
-constexpr int kMaxBlocks = 1024;  // workgroups of the forward = rows of partial counts
+// Workgroups of the forward a CU, as many as are resident at once (of four waves, one on each SIMD): four of at most 128
+// registers; three for 16 candidates of fp32 a lane and, for LDS, for the longest rows.  One round of them and no more: a second,
+// short round lasts as long as a full one (131072 x 256 with 768 resident: 1024 workgroups 104 us, 768 workgroups 87).
+constexpr int kCus = 256;
+constexpr int resident(int item_bytes, int lpr, int ipl) { return ipl == 16 && (lpr == 64 || item_bytes == 4) ? 3 : 4; }
 
 struct RouteParams {
   const void* logits;
@@ -56,13 +60,66 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k);
 }
 
+// exp in 64 bits, to 2 ulp: x = n ln 2 + r, |r| <= ln 2 / 2, the Taylor sum of r to r^13 / 13!.  Its constants are made where
+// they are used: the library's are kept in 22 registers over the whole loop over rows, of which almost none gets here.
+template <uint64_t kBits>
+__device__ __forceinline__ double constant() {
+  uint32_t lo, hi;
+  asm volatile("s_mov_b32 %0, %2\n\ts_mov_b32 %1, %3" : "=s"(lo), "=s"(hi) : "i"((uint32_t)kBits), "i"((uint32_t)(kBits >> 32)));
+  return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
+}
+#define UR_CONSTANT(value) constant<__builtin_bit_cast(uint64_t, (double)(value))>()
+__device__ __forceinline__ double exp64(double x) {
+  const double y = __builtin_fmin(__builtin_fmax(x, -1100.0), 1100.0), n = rint(y * UR_CONSTANT(1.4426950408889634));
+  const double r = __builtin_fma(n, UR_CONSTANT(-2.3190468138462996e-17), __builtin_fma(n, UR_CONSTANT(-0.6931471805599453), y));
+  double p = UR_CONSTANT(1.0 / 6227020800.0);
+  p = __builtin_fma(p, r, UR_CONSTANT(1.0 / 479001600.0));
+  p = __builtin_fma(p, r, UR_CONSTANT(1.0 / 39916800.0));
+  p = __builtin_fma(p, r, UR_CONSTANT(1.0 / 3628800.0));
+  p = __builtin_fma(p, r, UR_CONSTANT(1.0 / 362880.0));
+  p = __builtin_fma(p, r, UR_CONSTANT(1.0 / 40320.0));
+  p = __builtin_fma(p, r, UR_CONSTANT(1.0 / 5040.0));
+  p = __builtin_fma(p, r, UR_CONSTANT(1.0 / 720.0));
+  p = __builtin_fma(p, r, UR_CONSTANT(1.0 / 120.0));
+  p = __builtin_fma(p, r, UR_CONSTANT(1.0 / 24.0));
+  p = __builtin_fma(p, r, UR_CONSTANT(1.0 / 6.0));
+  p = __builtin_fma(p, r, 0.5);
+  p = __builtin_fma(p, r, 1.0);
+  p = __builtin_fma(p, r, 1.0);
+  return x != x ? x : ldexp(p, (int)n);
+}
+#undef UR_CONSTANT
+
+// Steps of a reduction over the wave as in reduce_lanes: what each lane gets to combine its value with.
+template <int kStep>
+__device__ __forceinline__ uint32_t wave_other(uint32_t v) {
+  if constexpr (kStep < 4) {
+    constexpr int kCtrl[4] = {kDppXor1, kDppXor2, kDppHalfMirror, kDppMirror};
+    return dpp32<kCtrl[kStep]>(v);
+  } else {
+    const auto r = kStep == 4 ? __builtin_amdgcn_permlane16_swap(v, v, false, false)
+                              : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return r[0] ^ r[1] ^ v;  // (one of the two is the lane's own)
+  }
+}
+template <int kStep = 0>
 __device__ __forceinline__ double wave_sum(double v) {
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  const uint64_t b = (uint64_t)__double_as_longlong(v);
+  const uint64_t o = ((uint64_t)wave_other<kStep>((uint32_t)(b >> 32)) << 32) | wave_other<kStep>((uint32_t)b);
+  v += __longlong_as_double((long long)o);
+  if constexpr (kStep < 5) v = wave_sum<kStep + 1>(v);
+  return v;
+}
+template <int kStep = 0>
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  v = max(v, wave_other<kStep>(v));
+  if constexpr (kStep < 5) v = wave_max<kStep + 1>(v);
   return v;
 }
 
 // ---- the choice in 64 bits, one wave for a row; lane j < k returns slot j's candidate or -1 --------------------------
-// `store`: LDS of this wave, 8 bytes a candidate: first the groups' values, then the keys.
+// `store`: LDS of this wave, 8 bytes a candidate: the keys.  Few rows come here, but a launch of few rows lasts as long as the
+// one that does: the maxima go through lane exchanges in registers.
 template <typename T>
 __device__ int choose_wide(const RouteParams& P, const T* __restrict__ row, uint64_t* store) {
   const int lane = threadIdx.x & 63, E = P.cands;
@@ -74,28 +131,26 @@ __device__ int choose_wide(const RouteParams& P, const T* __restrict__ row, uint
     mf = reduce_lanes<64, OpMax>(mf);
     m = mf == -__builtin_inff() ? 0.0 : (double)mf;
     z = 0.0;
-    for (int e = lane; e < E; e += 64) z += exp((double)(float)row[e] - m);
+    for (int e = lane; e < E; e += 64) z += exp64((double)(float)row[e] - m);
     z = wave_sum(z);
   }
-  // c of a candidate (by_score: s where c would be the bare logit), -inf where it is not eligible
-  const auto value = [&](int e, bool by_score) {
+  // key of a candidate's c (by_score: of s where c would be the bare logit), 0 where it is not eligible
+  const auto key = [&](int e, bool by_score) -> uint64_t {
     const double l = (double)(float)row[e];
-    if (l == -inf) return -inf;
-    if (!P.bias && !by_score) return l;
-    const double s = P.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - m) / z;
-    return P.bias ? s + (double)P.bias[e] : s;
+    if (l == -inf) return 0;
+    if (!P.bias && !by_score) return order_key(l);
+    const double s = P.sigmoid ? 1.0 / (1.0 + exp64(-l)) : exp64(l - m) / z;
+    const double c = P.bias ? s + (double)P.bias[e] : s;
+    return c == -inf ? 0 : order_key(c);
   };
   wave_lds_handoff();
-  uint64_t kept = ~0ull;
+  for (int e = lane; e < E; e += 64) store[e] = key(e, P.groups > 1 && P.top2);
+  wave_lds_handoff();
   if (P.groups > 1) {
-    for (int e = lane; e < E; e += 64) {
-      const double v = value(e, P.top2);
-      store[e] = v == -inf ? 0 : order_key(v);
-    }
-    wave_lds_handoff();
     uint64_t g = 0;
     if (lane < P.groups) {
       uint64_t a = 0, b = 0;  // the two largest (0: none)
+#pragma unroll 4
       for (int i = 0; i < P.per_group; ++i) {
         const uint64_t k = store[lane * P.per_group + i];
         b = k > a ? a : (k > b ? k : b);
@@ -105,17 +160,18 @@ __device__ int choose_wide(const RouteParams& P, const T* __restrict__ row, uint
     }
     int rank = 0;
     for (int o = 0; o < P.groups; ++o) {
-      const uint64_t other = __shfl(g, o);
+      const uint64_t other = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(g >> 32), o) << 32) |
+                             (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)g, o);
       rank += other > g || (other == g && o < lane);
     }
-    kept = __ballot(lane < P.groups && rank < P.top_groups);
+    const uint64_t kept = __ballot(lane < P.groups && rank < P.top_groups);
+    wave_lds_handoff();
+    for (int e = lane; e < E; e += 64) {
+      if (!((kept >> (e / P.per_group)) & 1)) store[e] = 0;
+      else if (!P.bias && P.top2) store[e] = key(e, false);
+    }
     wave_lds_handoff();
   }
-  for (int e = lane; e < E; e += 64) {
-    const double v = value(e, false);
-    store[e] = (v == -inf || (P.groups > 1 && !((kept >> (e / P.per_group)) & 1))) ? 0 : order_key(v);
-  }
-  wave_lds_handoff();
   int mine = -1;
   for (int r = 0; r < P.top_k; ++r) {
     uint64_t best = 0;
@@ -125,15 +181,12 @@ __device__ int choose_wide(const RouteParams& P, const T* __restrict__ row, uint
         best = store[e];
         at = e;
       }
-    for (int o = 32; o; o >>= 1) {
-      const uint64_t ob = __shfl_xor(best, o);
-      const int oa = __shfl_xor(at, o);
-      if (ob > best || (ob == best && oa < at)) {
-        best = ob;
-        at = oa;
-      }
-    }
-    if (best == 0) break;
+    // the largest key by halves, then the lowest index among those that hold it
+    const uint32_t hi = wave_max((uint32_t)(best >> 32));
+    const bool high = (uint32_t)(best >> 32) == hi;
+    const uint32_t lo = wave_max(high ? (uint32_t)best : 0);
+    if (hi == 0 && lo == 0) break;
+    at = kMaxCands - (int)wave_max(high && (uint32_t)best == lo ? (uint32_t)(kMaxCands - at) : 0);
     if (lane == r) mine = at;
     if ((at & 63) == lane) store[at] = 0;  // (read by this lane only)
   }
@@ -303,7 +356,7 @@ __device__ __forceinline__ Items<T, IPL> load_items(const T* __restrict__ row, i
 }
 
 template <typename T, int LPR, int IPL>
-__global__ void __launch_bounds__(kThreads, 3) k_route_fwd(const RouteParams P) {
+__global__ void __launch_bounds__(kThreads, resident(sizeof(T), LPR, IPL)) k_route_fwd(const RouteParams P) {
   constexpr int R = 64 / LPR, kRow = LPR * IPL;
   constexpr float kInf = __builtin_inff();
   __shared__ int hist[kRow];
@@ -471,7 +524,9 @@ __global__ void __launch_bounds__(kThreads, 3) k_route_fwd(const RouteParams P) 
         in_group = taken;
       } else {
         const uint64_t kept = (__ballot(taken) >> (sub * LPR));  // bit t: lane t's group is taken
-        int at = first / per, in = first % per;
+        int from = first;
+        asm("" : "+v"(from));  // (or the 16 places' groups are worked out before the loop over rows, and registers run out)
+        int at = from / per, in = from % per;
 #pragma unroll
         for (int i = 0; i < IPL; ++i) {
           if (at >= G || !((kept >> (at * share)) & 1)) c[i] = -kInf;
@@ -702,7 +757,7 @@ RouteShape route_shape(int cands, int top_k, int groups) {
   return s;
 }
 
-int route_parts(int64_t rows, int lpr) { return (int)std::min<int64_t>(ceil_div(rows, kWaves * (64 / lpr)), kMaxBlocks); }
+int route_parts(int64_t rows, int lpr, int most) { return (int)std::min<int64_t>(ceil_div(rows, kWaves * (64 / lpr)), kCus * most); }
 
 template <typename T>
 void launch_fwd(const RouteParams& P, RouteShape s, hipStream_t st) {
@@ -732,7 +787,7 @@ extern "C" {
 int64_t ur_route_workspace_bytes(int64_t rows, int cands) {
   if (rows <= 0 || cands <= 0 || rows > 0x7fffffff || cands > kMaxCands)
     return set_error(UR_ERR_INVALID_ARG, "bad rows or cands");
-  const int parts = route_parts(rows, 64);  // (the most any shape needs)
+  const int parts = route_parts(rows, 64, 4);  // (the most any shape needs)
   return parts > 1 ? (int64_t)parts * cands * 4 : 0;
 }
 
@@ -758,7 +813,7 @@ int ur_route_forward(const void* logits, int64_t row_stride, int dtype, const fl
   P.sigmoid = score == UR_SCORE_SIGMOID; P.top2 = group_score == UR_GROUP_TOP2; P.renormalize = renormalize != 0;
   P.scale = scale; P.weights = weights; P.indices = indices; P.counts = counts;
   const RouteShape shape = route_shape(cands, top_k, groups);
-  P.ws = static_cast<int32_t*>(workspace); P.parts = route_parts(rows, shape.lpr);
+  P.ws = static_cast<int32_t*>(workspace); P.parts = route_parts(rows, shape.lpr, resident(dtype_bytes(dtype), shape.lpr, shape.ipl));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == UR_F32) launch_fwd<float>(P, shape, st);
   else if (dtype == UR_F16) launch_fwd<_Float16>(P, shape, st);
