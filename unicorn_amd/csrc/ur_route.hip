@@ -11,6 +11,7 @@
 #include "ur_rows.h"
 
 #include <algorithm>
+#include <type_traits>
 
 using namespace ur;
 
@@ -18,10 +19,12 @@ namespace {
 
 constexpr int kMaxCands = 1024, kMaxTop = 64, kMaxGroups = 64;
 constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kSteps = 32;  // rounds of the forward between two looks at the rows that are to be chosen again
 typedef float f32x4_lds __attribute__((ext_vector_type(4)));
 // Workgroups of the forward a CU, as many as are resident at once (of four waves, one on each SIMD): four of at most 128
-// registers; three for 16 candidates of fp32 a lane and, for LDS, for the longest rows.  One round of them and no more: a second,
-// short round lasts as long as a full one (131072 x 256 with 768 resident: 1024 workgroups 104 us, 768 workgroups 87).
+// registers; three for 16 candidates of fp32 a lane and, for LDS, for the longest rows.  One round of them and no more: a
+// second, short round lasts as long as a full one (131072 x 256 with 768 resident: 1024 workgroups 104 us, 768 workgroups 87).
+// Five or six of fewer registers gain nothing (131072 x 64: 40 against 39 us): the forward is bound by instruction issue.
 constexpr int kCus = 256;
 constexpr int resident(int item_bytes, int lpr, int ipl) { return ipl == 16 && (lpr == 64 || item_bytes == 4) ? 3 : 4; }
 
@@ -246,11 +249,16 @@ __device__ __forceinline__ void row_softmax(const T* __restrict__ row, int E, in
 // ---- forward: LPR lanes a row, IPL consecutive candidates a lane -----------------------------------------------------
 // The choice is made in fp32 and redone in 64 bits (choose_wide) for the rows where fp32 cannot tell: with a bias, when two
 // neighbours of the order -- or the last group taken and the first one left -- are closer than fp32's error and are not the
-// same (logit, bias) twice.  Without a bias the logits themselves are compared and nothing has to be redone.
+// same (logit, bias) twice.  Without a bias the logits themselves are compared and nothing has to be redone.  Such rows are
+// noted and done after every kSteps rounds, outside the loop over rows, which has the registers to itself then.
+//
+// Bound by instruction issue, not by memory: 131072 rows of 256 bf16, sigmoid with bias and 4 of 8 groups, top 8: 75 us (67 MB
+// read: 0.9 TB/s), softmax without a bias 44 us; 4099 x 64: 11 us, most of it the latency of one row after the other that is
+// done in 64 bits.  All logits equal (every row is done in 64 bits): 567 us.
 //
 // The top-k is not taken by k rounds of a maximum: the (k+1)-th largest of the lanes' maxima is a lower bound of the (k+1)-th
-// largest candidate; the few candidates that reach it (about 10 of 256) go to a list in LDS as (key, index) and each finds its rank
-// by counting the larger ones.
+// largest candidate; the few candidates that reach it (about 10 of 256) go to a list in LDS as (key, index) and each finds
+// its rank by counting the larger ones.
 
 // how many of the values that a row's other 15 lanes hold (two a lane) are >= v, >= w
 template <int kRor>
@@ -343,17 +351,33 @@ __device__ __forceinline__ int count_larger16(uint32_t hi, uint32_t lo) {
 // the hardware's exponential (1 ulp) of the argument rounded to base 2
 __device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
 
-// IPL consecutive logits, as they are stored; -inf behind the row's end
+// IPL consecutive numbers of a row, as they are stored, in whole registers (of 16-bit ones a register each is taken otherwise)
 template <typename T, int IPL>
-struct __attribute__((packed, aligned(sizeof(T)))) Items { T v[IPL]; };
-template <typename T, int IPL>
-__device__ __forceinline__ Items<T, IPL> load_items(const T* __restrict__ row, int first, int E) {
-  if (first + IPL <= E) return *reinterpret_cast<const Items<T, IPL>*>(row + first);
-  Items<T, IPL> it;
+struct Items {
+  using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+  static constexpr int kPer = sizeof(T) == 4 || IPL == 1 ? 1 : 2, kWords = IPL / kPer;
+  struct __attribute__((packed, aligned(sizeof(T)))) Stored { std::conditional_t<kPer == 2, uint32_t, Bits> w[kWords]; };
+  uint32_t w[kWords];
+  // from column `first`; `fill` behind the row's end
+  __device__ __forceinline__ void load(const T* __restrict__ row, int first, int E, T fill) {
+    if (first + IPL <= E) {
+      const Stored s = *reinterpret_cast<const Stored*>(row + first);
 #pragma unroll
-  for (int i = 0; i < IPL; ++i) it.v[i] = first + i < E ? row[first + i] : (T)-__builtin_inff();
-  return it;
-}
+      for (int i = 0; i < kWords; ++i) w[i] = s.w[i];
+      return;
+    }
+    const Bits* in = reinterpret_cast<const Bits*>(row);
+    const uint32_t none = __builtin_bit_cast(Bits, fill);
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      w[i] = first + i * kPer < E ? in[first + i * kPer] : none;
+      if constexpr (kPer == 2) w[i] |= (first + i * 2 + 1 < E ? in[first + i * 2 + 1] : none) << 16;
+    }
+  }
+  __device__ __forceinline__ float operator[](int i) const {
+    return (float)__builtin_bit_cast(T, (Bits)(w[i / kPer] >> (kPer == 2 ? 16 * (i & 1) : 0)));
+  }
+};
 
 template <typename T, int LPR, int IPL>
 __global__ void __launch_bounds__(kThreads, resident(sizeof(T), LPR, IPL)) k_route_fwd(const RouteParams P) {
@@ -364,12 +388,15 @@ __global__ void __launch_bounds__(kThreads, resident(sizeof(T), LPR, IPL)) k_rou
   __shared__ uint64_t store[kWaves][R * kRow / 2 > kRow ? R * kRow / 2 : kRow];
   __shared__ uint16_t lists[kWaves][R * kRow];  // candidates that reach the bound
   __shared__ uint64_t slot_store[kWaves][R * (LPR + 1)];
+  __shared__ uint32_t redo_rows[kSteps * kWaves * R];
+  __shared__ int redo_count[2];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / LPR, t = lane % LPR;
   float* vals = reinterpret_cast<float*>(store[wave]) + sub * kRow;
   uint16_t* list = lists[wave] + sub * kRow;
   uint64_t* slots = slot_store[wave] + sub * (LPR + 1);
   const int E = P.cands, first = t * IPL, k = P.top_k, G = P.groups, per = P.per_group;
   for (int e = threadIdx.x; e < E; e += kThreads) hist[e] = 0;
+  if (threadIdx.x < 2) redo_count[threadIdx.x] = 0;
   __syncthreads();
   const bool group_scores = G > 1 && P.top2 && !P.bias;  // groups are compared by sums of scores, candidates by logits
   const bool need_scores = P.bias != nullptr || group_scores;
@@ -381,7 +408,13 @@ __global__ void __launch_bounds__(kThreads, resident(sizeof(T), LPR, IPL)) k_rou
   while (share > 1 && LPR / share < G) share >>= 1;
   float bias[IPL];
 #pragma unroll
-  for (int i = 0; i < IPL; ++i) bias[i] = (P.bias && first + i < E) ? P.bias[first + i] : 0.0f;
+  for (int i = 0; i < IPL; ++i) bias[i] = 0.0f;
+  if (P.bias) {
+    Items<float, IPL> b;
+    b.load(P.bias, first, E, 0.0f);
+#pragma unroll
+    for (int i = 0; i < IPL; ++i) bias[i] = b[i];
+  }
 
   bool odd_bias = false;  // infinities or NaN among the biases
 #pragma unroll
@@ -391,262 +424,282 @@ __global__ void __launch_bounds__(kThreads, resident(sizeof(T), LPR, IPL)) k_rou
   const uint32_t last = (uint32_t)P.rows - 1, per_step = kWaves * R, row_groups = last / per_step + 1;
   const auto row_at = [&](uint32_t row) { return static_cast<const T*>(P.logits) + (uint64_t)row * (uint64_t)P.stride; };
   uint32_t row = min(blockIdx.x * per_step + wave * R + sub, last);
-  Items<T, IPL> ahead = load_items<T, IPL>(row_at(row), first, E);
-  for (uint32_t rg = blockIdx.x; rg < row_groups; rg += gridDim.x) {
-    const uint32_t want = rg * per_step + wave * R + sub;
-    const bool mine = want <= last;
-    row = min(want, last);
-    const T* src = row_at(row);
-    float c[IPL];  // logits, then what the candidates are compared by; -inf: not eligible
-    float probe = 0.0f;
+  constexpr T kNone = (T)-__builtin_inff();
+  Items<T, IPL> ahead;
+  ahead.load(row_at(row), first, E, kNone);
+  int flip = 0;
+  for (uint32_t rg0 = blockIdx.x; rg0 < row_groups; rg0 += kSteps * gridDim.x) {
+    for (uint32_t rg = rg0; rg < min(rg0 + kSteps * gridDim.x, row_groups); rg += gridDim.x) {
+      const uint32_t want = rg * per_step + wave * R + sub;
+      const bool mine = want <= last;
+      row = min(want, last);
+      const T* src = row_at(row);
+      float c[IPL];  // logits, then what the candidates are compared by; -inf: not eligible
+      float probe = 0.0f;
 #pragma unroll
-    for (int i = 0; i < IPL; ++i) {
-      c[i] = (float)ahead.v[i];
-      probe = __builtin_fmaf(c[i], 0.0f, probe);  // NaN as soon as one logit is not finite
-    }
-    const bool odd = odd_bias || __any(probe != probe);  // (E not a multiple of IPL: the places behind the end are -inf)
-    ahead = load_items<T, IPL>(row_at(min((rg + gridDim.x) * per_step + wave * R + sub, last)), first, E);
-
-    // err: bound of two scores' errors.  sigmoid: s (1 - s) (|l| 2^-23.4 + 2^-23) of the exponential, 2^-23 of the
-    // reciprocal, 2^-24 of the sum: below 2^-22 each.  softmax, relative to its largest score 1 / z: as much of the
-    // exponential and up to 30 roundings of z, below 2^-19 each.
-    float m = 0.0f, z = 1.0f, inv_z = 1.0f, err = 0x1p-20f;
-    if (need_softmax) {
-      float mf = c[0];
-#pragma unroll
-      for (int i = 1; i < IPL; ++i) mf = __builtin_fmaxf(mf, c[i]);
-      mf = reduce_lanes<LPR, OpMax>(mf);
-      m = mf == -kInf ? 0.0f : mf;
-      float sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < IPL; ++i) sum += fast_exp(c[i] - m);
-      z = reduce_lanes<LPR, OpSum>(sum);
-      if (z == 0.0f) z = 1.0f;
-      inv_z = 1.0f / z;
-      err = 0x1p-17f * inv_z;
-    }
-    float a = -kInf, b = -kInf;  // the two largest of this lane's part of its group
-    if (need_scores) {
-      float s[IPL];
-      if (P.sigmoid) {
-#pragma unroll
-        for (int i = 0; i < IPL; ++i) s[i] = __builtin_amdgcn_rcpf(1.0f + fast_exp(-c[i]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < IPL; ++i) s[i] = fast_exp(c[i] - m) * inv_z;
+      for (int i = 0; i < IPL; ++i) {
+        c[i] = ahead[i];
+        probe = __builtin_fmaf(c[i], 0.0f, probe);  // NaN as soon as one logit is not finite
       }
-      if (P.bias) {
-#pragma unroll
-        for (int i = 0; i < IPL; ++i) s[i] += bias[i];
-        if (odd) {
-#pragma unroll
-          for (int i = 0; i < IPL; ++i) s[i] = c[i] == -kInf ? -kInf : s[i];
-        }
-#pragma unroll
-        for (int i = 0; i < IPL; ++i) c[i] = s[i];
-      } else {  // the groups' values are of the scores
-#pragma unroll
-        for (int i = 0; i < IPL; ++i) {
-          s[i] = c[i] == -kInf ? -kInf : s[i] != s[i] ? kInf : s[i];
-          if (!whole) vals[first + i] = s[i];
-          const float lo = __builtin_fminf(a, s[i]);
-          a = __builtin_fmaxf(a, s[i]);
-          b = __builtin_fmaxf(b, lo);
-        }
-      }
-    }
-    if (odd) {
-#pragma unroll
-      for (int i = 0; i < IPL; ++i) c[i] = c[i] != c[i] ? kInf : c[i];
-    }
+      const bool odd = odd_bias || __any(probe != probe);  // (E not a multiple of IPL: the places behind the end are -inf)
+      ahead.load(row_at(min((rg + gridDim.x) * per_step + wave * R + sub, last)), first, E, kNone);
 
-    bool close = false;  // fp32 cannot tell
-    bool in_group = true;  // (whole groups of lanes) this lane's group is taken
-    if (G > 1) {
-      if (!group_scores) {
-        if (whole && !P.top2) {
+      // err: bound of two scores' errors.  sigmoid: s (1 - s) (|l| 2^-23.4 + 2^-23) of the exponential, 2^-23 of the
+      // reciprocal, 2^-24 of the sum: below 2^-22 each.  softmax, relative to its largest score 1 / z: as much of the
+      // exponential and up to 30 roundings of z, below 2^-19 each.
+      float m = 0.0f, z = 1.0f, inv_z = 1.0f, err = 0x1p-20f;
+      if (need_softmax) {
+        float mf = c[0];
 #pragma unroll
-          for (int i = 0; i < IPL; ++i) a = __builtin_fmaxf(a, c[i]);
-        } else if (whole) {
+        for (int i = 1; i < IPL; ++i) mf = __builtin_fmaxf(mf, c[i]);
+        mf = reduce_lanes<LPR, OpMax>(mf);
+        m = mf == -kInf ? 0.0f : mf;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < IPL; ++i) sum += fast_exp(c[i] - m);
+        z = reduce_lanes<LPR, OpSum>(sum);
+        if (z == 0.0f) z = 1.0f;
+        inv_z = 1.0f / z;
+        err = 0x1p-17f * inv_z;
+      }
+      float a = -kInf, b = -kInf;  // the two largest of this lane's part of its group
+      if (need_scores) {
+        float s[IPL];
+        if (P.sigmoid) {
+#pragma unroll
+          for (int i = 0; i < IPL; ++i) s[i] = __builtin_amdgcn_rcpf(1.0f + fast_exp(-c[i]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < IPL; ++i) s[i] = fast_exp(c[i] - m) * inv_z;
+        }
+        if (P.bias) {
+#pragma unroll
+          for (int i = 0; i < IPL; ++i) s[i] += bias[i];
+          if (odd) {
+#pragma unroll
+            for (int i = 0; i < IPL; ++i) s[i] = c[i] == -kInf ? -kInf : s[i];
+          }
+#pragma unroll
+          for (int i = 0; i < IPL; ++i) c[i] = s[i];
+        } else {  // the groups' values are of the scores
 #pragma unroll
           for (int i = 0; i < IPL; ++i) {
-            const float lo = __builtin_fminf(a, c[i]);
-            a = __builtin_fmaxf(a, c[i]);
+            s[i] = c[i] == -kInf ? -kInf : s[i] != s[i] ? kInf : s[i];
+            if (!whole) vals[first + i] = s[i];
+            const float lo = __builtin_fminf(a, s[i]);
+            a = __builtin_fmaxf(a, s[i]);
             b = __builtin_fmaxf(b, lo);
           }
-        } else {
+        }
+      }
+      if (odd) {
+#pragma unroll
+        for (int i = 0; i < IPL; ++i) c[i] = c[i] != c[i] ? kInf : c[i];
+      }
+
+      bool close = false;  // fp32 cannot tell
+      bool in_group = true;  // (whole groups of lanes) this lane's group is taken
+      if (G > 1) {
+        if (!group_scores) {
+          if (whole && !P.top2) {
+#pragma unroll
+            for (int i = 0; i < IPL; ++i) a = __builtin_fmaxf(a, c[i]);
+          } else if (whole) {
+#pragma unroll
+            for (int i = 0; i < IPL; ++i) {
+              const float lo = __builtin_fminf(a, c[i]);
+              a = __builtin_fmaxf(a, c[i]);
+              b = __builtin_fmaxf(b, lo);
+            }
+          } else {
+            wave_lds_handoff();
+#pragma unroll
+            for (int i = 0; i < IPL; ++i) vals[first + i] = c[i];
+          }
+        }
+        const int width = whole ? lanes_per : share;  // lanes that hold the same group
+        if (!whole) {
           wave_lds_handoff();
-#pragma unroll
-          for (int i = 0; i < IPL; ++i) vals[first + i] = c[i];
+          const int g = t / share;
+          a = b = -kInf;
+          if (g < G)
+            for (int i = t % share; i < per; i += share) {
+              const float v = vals[g * per + i], lo = __builtin_fminf(a, v);
+              a = __builtin_fmaxf(a, v);
+              b = __builtin_fmaxf(b, lo);
+            }
         }
-      }
-      const int width = whole ? lanes_per : share;  // lanes that hold the same group
-      if (!whole) {
-        wave_lds_handoff();
-        const int g = t / share;
-        a = b = -kInf;
-        if (g < G)
-          for (int i = t % share; i < per; i += share) {
-            const float v = vals[g * per + i], lo = __builtin_fminf(a, v);
-            a = __builtin_fmaxf(a, v);
-            b = __builtin_fmaxf(b, lo);
-          }
-      }
-      for (int o = 1; o < width; o <<= 1) {
-        const float a2 = __shfl_xor(a, o), b2 = __shfl_xor(b, o);
-        b = __builtin_fmaxf(__builtin_fminf(a, a2), __builtin_fmaxf(b, b2));
-        a = __builtin_fmaxf(a, a2);
-      }
-      // (two biases of the lowest number stay above a group that nothing is eligible of)
-      const float g = P.top2 && b != -kInf ? __builtin_fmaxf(a + b, -__FLT_MAX__) : a;
-      const int my_group = t / width;
-      // by (value, lower index): a group's rank is the number of groups before it
-      const uint32_t hi = order_key(g), lo = (uint32_t)(kMaxGroups - my_group);
-      int rank = 0;
-      for (int o = 0; o < G; o += 4) {
-        uint32_t other[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) other[i] = (uint32_t)__shfl((int)hi, min(o + i, G - 1) * width, LPR);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint64_t mine_key = ((uint64_t)hi << 32) | lo;
-          rank += o + i < G && (((uint64_t)other[i] << 32) | (uint32_t)(kMaxGroups - o - i)) > mine_key;
+        for (int o = 1; o < width; o <<= 1) {
+          const float a2 = __shfl_xor(a, o), b2 = __shfl_xor(b, o);
+          b = __builtin_fmaxf(__builtin_fminf(a, a2), __builtin_fmaxf(b, b2));
+          a = __builtin_fmaxf(a, a2);
         }
-      }
-      const bool taken = my_group < G && rank < P.top_groups;
-      if (need_scores && P.top_groups < G) {  // the last group taken against the first one left
-        const uint64_t at_last = __ballot(my_group < G && rank == P.top_groups - 1) >> (sub * LPR);
-        const float worst = __shfl(g, __builtin_ctzll(at_last), LPR);
-        if (my_group < G && rank == P.top_groups && g != -kInf)
-          close = !(worst - g > 2.0f * err + 0x1p-21f * (fabsf(worst) + fabsf(g)));  // (inf - inf: cannot tell)
-      }
-      if (whole) {
-        in_group = taken;
-      } else {
-        const uint64_t kept = (__ballot(taken) >> (sub * LPR));  // bit t: lane t's group is taken
-        int from = first;
-        asm("" : "+v"(from));  // (or the 16 places' groups are worked out before the loop over rows, and registers run out)
-        int at = from / per, in = from % per;
-#pragma unroll
-        for (int i = 0; i < IPL; ++i) {
-          if (at >= G || !((kept >> (at * share)) & 1)) c[i] = -kInf;
-          if (++in == per) {
-            in = 0;
-            ++at;
-          }
-        }
-      }
-    }
-
-    // the candidates that can be among the k + 1 largest: their places in a list, their values in LDS
-    float bound = -__FLT_MAX__;
-    if constexpr (IPL > 1) {
-      float v = c[0], w = c[IPL / 2];
-#pragma unroll
-      for (int i = 1; i < IPL / 2; ++i) {
-        v = __builtin_fmaxf(v, c[i]);
-        w = __builtin_fmaxf(w, c[IPL / 2 + i]);
-      }
-      bound = prune_bound<LPR>(in_group ? v : -kInf, in_group ? w : -kInf, k);
-    }
-    uint32_t reach = 0;
-#pragma unroll
-    for (int i = IPL - 1; i >= 0; --i) reach = 2 * reach + (c[i] >= bound);
-    if (!in_group) reach = 0;
-    wave_lds_handoff();
-#pragma unroll
-    for (int i = 0; i < IPL; ++i) vals[first + i] = c[i];
-    int before = lanes_before<LPR>(__popc(reach), t);
-    int n = __shfl(before + __popc(reach), LPR - 1, LPR);
-    if (__any(n > 2 * LPR)) {  // many equal values: of those at the bound the first k + 1 will do
-      uint32_t larger = 0;
-#pragma unroll
-      for (int i = IPL - 1; i >= 0; --i) larger = 2 * larger + (c[i] > bound);
-      larger &= reach;
-      uint32_t equal = reach & ~larger, kept = 0;
-      int left = k + 1 - lanes_before<LPR>(__popc(equal), t);
-      for (; equal && left > 0; --left, equal &= equal - 1) kept |= equal & (0u - equal);
-      reach = larger | kept;
-      before = lanes_before<LPR>(__popc(reach), t);
-      n = __shfl(before + __popc(reach), LPR - 1, LPR);
-    }
-    for (; reach; reach &= reach - 1) list[before++] = (uint16_t)(first + __builtin_ctz(reach));
-    for (int j = t; j <= k; j += LPR) slots[j] = 0;
-    wave_lds_handoff();
-    const auto entry = [&](int j) {
-      const int e = list[j];
-      return ((uint64_t)order_key(vals[e]) << 32) | (uint32_t)(kMaxCands - e);  // (of equal values the lower index is larger)
-    };
-    uint64_t own = t < n ? entry(t) : 0;
-    int n_max = n;
-    if constexpr (R > 1) n_max = (int)reduce_lanes<64, OpMax>((float)n);
-    constexpr int kPer = IPL < 8 ? (IPL > 1 ? IPL / 2 : 1) : 4;  // entries a lane that fit over the values
-    if (n_max <= LPR) {
-      int rank = 0;
-      if constexpr (LPR == 16) {
-        rank = count_larger16<15>((uint32_t)(own >> 32), (uint32_t)own);
-      } else {
-        const float hi = __uint_as_float((uint32_t)(own >> 32)), lo = __uint_as_float((uint32_t)own);
-        for (int i = 0; i < n_max; ++i)
-          rank += (((uint64_t)__float_as_uint(row_lane<LPR>(hi, i)) << 32) | __float_as_uint(row_lane<LPR>(lo, i))) > own;
-      }
-      if (own && rank <= k) slots[rank] = own;
-    } else if (n_max <= kPer * LPR) {
-      uint64_t mine_all[kPer];
-#pragma unroll
-      for (int q = 0; q < kPer; ++q) mine_all[q] = t + q * LPR < n ? entry(t + q * LPR) : 0;
-      wave_lds_handoff();
-      uint64_t* entries = store[wave] + sub * (kPer * LPR);
-#pragma unroll
-      for (int q = 0; q < kPer; ++q) entries[t + q * LPR] = mine_all[q];
-      wave_lds_handoff();
-      int rank[kPer] = {};
-#pragma unroll 2
-      for (int i = 0; i < n_max; ++i) {
-        const uint64_t other = entries[i];
-#pragma unroll
-        for (int q = 0; q < kPer; ++q) rank[q] += other > mine_all[q];
-      }
-#pragma unroll
-      for (int q = 0; q < kPer; ++q)
-        if (mine_all[q] && rank[q] <= k) slots[rank[q]] = mine_all[q];
-    } else {
-      for (int j = t; j < n; j += LPR) {
-        own = entry(j);
+        // (two biases of the lowest number stay above a group that nothing is eligible of)
+        const float g = P.top2 && b != -kInf ? __builtin_fmaxf(a + b, -__FLT_MAX__) : a;
+        const int my_group = t / width;
+        // by (value, lower index): a group's rank is the number of groups before it
+        const uint32_t hi = order_key(g), lo = (uint32_t)(kMaxGroups - my_group);
         int rank = 0;
-        for (int i = 0; i < n; ++i) rank += entry(i) > own;
-        if (rank <= k) slots[rank] = own;
+        for (int o = 0; o < G; o += 4) {
+          uint32_t other[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) other[i] = (uint32_t)__shfl((int)hi, min(o + i, G - 1) * width, LPR);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint64_t mine_key = ((uint64_t)hi << 32) | lo;
+            rank += o + i < G && (((uint64_t)other[i] << 32) | (uint32_t)(kMaxGroups - o - i)) > mine_key;
+          }
+        }
+        const bool taken = my_group < G && rank < P.top_groups;
+        if (need_scores && P.top_groups < G) {  // the last group taken against the first one left
+          const uint64_t at_last = __ballot(my_group < G && rank == P.top_groups - 1) >> (sub * LPR);
+          const float worst = __shfl(g, __builtin_ctzll(at_last), LPR);
+          if (my_group < G && rank == P.top_groups && g != -kInf)
+            close = !(worst - g > 2.0f * err + 0x1p-21f * (fabsf(worst) + fabsf(g)));  // (inf - inf: cannot tell)
+        }
+        if (whole) {
+          in_group = taken;
+        } else {
+          const uint64_t kept = (__ballot(taken) >> (sub * LPR));  // bit t: lane t's group is taken
+          int from = first;
+          asm("" : "+v"(from));  // (or the 16 places' groups are worked out before the loop over rows, and registers run out)
+          int at = from / per, in = from % per;
+#pragma unroll
+          for (int i = 0; i < IPL; ++i) {
+            if (at >= G || !((kept >> (at * share)) & 1)) c[i] = -kInf;
+            if (++in == per) {
+              in = 0;
+              ++at;
+            }
+          }
+        }
       }
-    }
-    wave_lds_handoff();
 
-    const uint64_t got = t < k ? slots[t] : 0;
-    int at = got ? kMaxCands - (int)(uint32_t)got : -1;
-    if (P.bias && got) {
-      const uint64_t next = slots[t + 1];
-      const float v = key_value((uint32_t)(got >> 32)), v2 = key_value((uint32_t)(next >> 32));
-      if (next && v - v2 <= err + 0x1p-22f * (fabsf(v) + fabsf(v2))) {
-        const int at2 = kMaxCands - (int)(uint32_t)next;
-        close |= !((float)src[at] == (float)src[at2] && P.bias[at] == P.bias[at2]);
+      // the candidates that can be among the k + 1 largest: their places in a list, their values in LDS
+      float bound = -__FLT_MAX__;
+      if constexpr (IPL > 1) {
+        float v = c[0], w = c[IPL / 2];
+#pragma unroll
+        for (int i = 1; i < IPL / 2; ++i) {
+          v = __builtin_fmaxf(v, c[i]);
+          w = __builtin_fmaxf(w, c[IPL / 2 + i]);
+        }
+        bound = prune_bound<LPR>(in_group ? v : -kInf, in_group ? w : -kInf, k);
       }
-    }
-    uint64_t redo = __ballot(close && mine);
-    while (redo) {  // (the whole wave, one row at a time)
-      const int r = __builtin_ctzll(redo) / LPR;
-      const int chosen = choose_wide<T>(P, row_at(rg * per_step + wave * R + r), store[wave]);
-      if (lane < k) slot_store[wave][r * (LPR + 1) + lane] = chosen < 0 ? 0 : (uint64_t)(kMaxCands - chosen);
+      uint32_t reach = 0;
+#pragma unroll
+      for (int i = IPL - 1; i >= 0; --i) reach = 2 * reach + (c[i] >= bound);
+      if (!in_group) reach = 0;
       wave_lds_handoff();
-      if (sub == r && t < k) at = slots[t] ? kMaxCands - (int)(uint32_t)slots[t] : -1;
-      redo &= R == 1 ? 0ull : ~(((1ull << (LPR & 63)) - 1) << (r * LPR));
-    }
+#pragma unroll
+      for (int i = 0; i < IPL; ++i) vals[first + i] = c[i];
+      int before = lanes_before<LPR>(__popc(reach), t);
+      int n = __shfl(before + __popc(reach), LPR - 1, LPR);
+      if (__any(n > 2 * LPR)) {  // many equal values: of those at the bound the first k + 1 will do
+        uint32_t larger = 0;
+#pragma unroll
+        for (int i = IPL - 1; i >= 0; --i) larger = 2 * larger + (c[i] > bound);
+        larger &= reach;
+        uint32_t equal = reach & ~larger, kept = 0;
+        int left = k + 1 - lanes_before<LPR>(__popc(equal), t);
+        for (; equal && left > 0; --left, equal &= equal - 1) kept |= equal & (0u - equal);
+        reach = larger | kept;
+        before = lanes_before<LPR>(__popc(reach), t);
+        n = __shfl(before + __popc(reach), LPR - 1, LPR);
+      }
+      for (; reach; reach &= reach - 1) list[before++] = (uint16_t)(first + __builtin_ctz(reach));
+      for (int j = t; j <= k; j += LPR) slots[j] = 0;
+      wave_lds_handoff();
+      const auto entry = [&](int j) {
+        const int e = list[j];
+        return ((uint64_t)order_key(vals[e]) << 32) | (uint32_t)(kMaxCands - e);  // (of equal values the lower index is larger)
+      };
+      uint64_t own = t < n ? entry(t) : 0;
+      int n_max = n;
+      if constexpr (R > 1) n_max = (int)reduce_lanes<64, OpMax>((float)n);
+      constexpr int kPer = IPL < 8 ? (IPL > 1 ? IPL / 2 : 1) : 4;  // entries a lane that fit over the values
+      if (n_max <= LPR) {
+        int rank = 0;
+        if constexpr (LPR == 16) {
+          rank = count_larger16<15>((uint32_t)(own >> 32), (uint32_t)own);
+        } else {
+          const float hi = __uint_as_float((uint32_t)(own >> 32)), lo = __uint_as_float((uint32_t)own);
+          for (int i = 0; i < n_max; ++i)
+            rank += (((uint64_t)__float_as_uint(row_lane<LPR>(hi, i)) << 32) | __float_as_uint(row_lane<LPR>(lo, i))) > own;
+        }
+        if (own && rank <= k) slots[rank] = own;
+      } else if (n_max <= kPer * LPR) {
+        uint64_t mine_all[kPer];
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) mine_all[q] = t + q * LPR < n ? entry(t + q * LPR) : 0;
+        wave_lds_handoff();
+        uint64_t* entries = store[wave] + sub * (kPer * LPR);
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) entries[t + q * LPR] = mine_all[q];
+        wave_lds_handoff();
+        int rank[kPer] = {};
+#pragma unroll 2
+        for (int i = 0; i < n_max; ++i) {
+          const uint64_t other = entries[i];
+#pragma unroll
+          for (int q = 0; q < kPer; ++q) rank[q] += other > mine_all[q];
+        }
+#pragma unroll
+        for (int q = 0; q < kPer; ++q)
+          if (mine_all[q] && rank[q] <= k) slots[rank[q]] = mine_all[q];
+      } else {
+        for (int j = t; j < n; j += LPR) {
+          own = entry(j);
+          int rank = 0;
+          for (int i = 0; i < n; ++i) rank += entry(i) > own;
+          if (rank <= k) slots[rank] = own;
+        }
+      }
+      wave_lds_handoff();
 
-    const Chosen ch = chosen_share<LPR>(P.sigmoid, P.renormalize, at >= 0 ? (float)src[at] : 0.0f, at >= 0, m, z);
-    if (mine && t < k) {
-      const uint64_t out = (uint64_t)row * (uint32_t)k + t;
-      P.weights[out] = z != z ? z : P.scale * ch.share;  // (a NaN in a softmax is in every score)
-      P.indices[out] = at;
-      if (at >= 0) atomicAdd(&hist[at], 1);
+      const uint64_t got = t < k ? slots[t] : 0;
+      const int at = got ? kMaxCands - (int)(uint32_t)got : -1;
+      if (P.bias && got) {
+        const uint64_t next = slots[t + 1];
+        const float v = key_value((uint32_t)(got >> 32)), v2 = key_value((uint32_t)(next >> 32));
+        if (next && v - v2 <= err + 0x1p-22f * (fabsf(v) + fabsf(v2))) {
+          const int at2 = kMaxCands - (int)(uint32_t)next;
+          close |= !((float)src[at] == (float)src[at2] && P.bias[at] == P.bias[at2]);
+        }
+      }
+      const uint64_t all_close = __ballot(close && mine);
+      const bool redo = R == 1 ? all_close != 0 : ((all_close >> (sub * LPR)) & ((1ull << (LPR & 63)) - 1)) != 0;
+      if (redo && t == 0) redo_rows[atomicAdd(&redo_count[flip], 1)] = row;
+
+      const Chosen ch = chosen_share<LPR>(P.sigmoid, P.renormalize, at >= 0 ? (float)src[at] : 0.0f, at >= 0, m, z);
+      if (mine && t < k && !redo) {
+        const uint64_t out = (uint64_t)row * (uint32_t)k + t;
+        P.weights[out] = z != z ? z : P.scale * ch.share;  // (a NaN in a softmax is in every score)
+        P.indices[out] = at;
+        if (at >= 0) atomicAdd(&hist[at], 1);
+      }
     }
+    // the rows that fp32 could not tell, a wave each
+    if (!need_scores) continue;
+    __syncthreads();
+    const int n_redo = redo_count[flip];
+    flip ^= 1;
+    if (threadIdx.x == 0) redo_count[flip] = 0;
+    for (int i = wave; i < n_redo; i += kWaves) {
+      const uint32_t again = redo_rows[i];
+      const T* src = row_at(again);
+      const int at = choose_wide<T>(P, src, store[wave]);
+      float m = 0.0f, z = 1.0f;
+      if (!P.sigmoid) row_softmax<T, 64>(src, E, lane, m, z);
+      const Chosen ch = chosen_share<64>(P.sigmoid, P.renormalize, at >= 0 ? (float)src[at] : 0.0f, at >= 0, m, z);
+      if (lane < k) {
+        const uint64_t out = (uint64_t)again * (uint32_t)k + lane;
+        P.weights[out] = z != z ? z : P.scale * ch.share;
+        P.indices[out] = at;
+        if (at >= 0) atomicAdd(&hist[at], 1);
+      }
+    }
+    __syncthreads();
   }
   __syncthreads();
   int32_t* out = P.parts > 1 ? P.ws + (int64_t)blockIdx.x * E : P.counts;
