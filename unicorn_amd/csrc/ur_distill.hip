@@ -98,6 +98,19 @@ __device__ __forceinline__ void add_batch(const typename Elem<T>::Vec (&v)[B], f
   for (int b = 0; b < B; ++b) s += part[b];
 }
 
+// The vector at `col` of a range that ends at c1 and holds at least one vector: where it would reach over the end it is moved
+// back to end there, and what belongs to the vector before it reads as `fill`.
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::Vec load_back(const T* __restrict__ z, int64_t col, int64_t c1, T fill) {
+  constexpr int N = Elem<T>::kN;
+  const int64_t at = min(col, c1 - N);
+  auto v = *reinterpret_cast<const typename Elem<T>::Vec*>(z + at);
+  const int skip = (int)min(col - at, (int64_t)N);
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = j < skip ? fill : v[j];
+  return v;
+}
+
 template <typename T, int B>
 __device__ __forceinline__ void row_part(const T* __restrict__ z, int64_t c0, int64_t c1, int t, int n, float scale, float& m,
                                          float& s) {
@@ -111,6 +124,9 @@ __device__ __forceinline__ void row_part(const T* __restrict__ z, int64_t c0, in
     if (col + (B - 1) * step + N <= c1) {
 #pragma unroll
       for (int b = 0; b < B; ++b) v[b] = *reinterpret_cast<const Vec*>(z + col + b * step);
+    } else if (c1 - c0 >= N) {
+#pragma unroll
+      for (int b = 0; b < B; ++b) v[b] = load_back<T>(z, col + b * step, c1, (T)-__builtin_inff());
     } else {
 #pragma unroll
       for (int b = 0; b < B; ++b) v[b] = load16<T>(z, col + b * step, c1, (T)-__builtin_inff());
@@ -415,6 +431,17 @@ __device__ __forceinline__ void write_q(const RowGrad& r, const T* __restrict__ 
   }
   if (col >= c1) return;
   Vec v[B];
+  if (c1 - c0 >= N) {  // (a vector moved back to the end writes some places twice, with the same numbers)
+#pragma unroll
+    for (int b = 0; b < B; ++b) v[b] = *reinterpret_cast<const Vec*>(z + min(col + b * step, c1 - N));
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[b][j] = r.zero ? (T)0.0f : (T)(r.g * r.q((float)v[b][j]));
+      if (col + b * step < c1) *reinterpret_cast<Vec*>(out + min(col + b * step, c1 - N)) = v[b];
+    }
+    return;
+  }
 #pragma unroll
   for (int b = 0; b < B; ++b) v[b] = load16<T>(z, col + b * step, c1, (T)0.0f);
 #pragma unroll
