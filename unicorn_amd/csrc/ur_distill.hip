@@ -32,7 +32,7 @@ struct DistillParams {
   int top;
   double temperature;
   float scale;     // log2(e) / T
-  double scale64;  // the same in 64 bits
+  double scale64, inv_t;  // the same in 64 bits; 1 / T
   float* stats;  // (rows, 2): maximum of z, sum of exp((z - max) / T)
   float* loss;   // (rows) or one value
   int reduction;
@@ -144,11 +144,6 @@ __device__ __forceinline__ void merge_lanes(float& m, float& s, float scale) {
 }
 
 template <int L>
-__device__ __forceinline__ double sum_lanes(double v) {
-  for (int o = L / 2; o; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-template <int L>
 __device__ __forceinline__ bool any_lane(bool v) {
   const uint64_t b = __ballot(v);
   if (L == 64) return b != 0;
@@ -174,21 +169,22 @@ __device__ __forceinline__ Slot slot_at(const DistillParams& P, int64_t row, con
 
 // The teacher of a row, by L lanes: maximum and sum of exponentials of its filled slots, and whether there is one; a class
 // outside [0, V) makes the sum NaN.  `own`: slot threadIdx.x % L, fetched before the row was read (its two dependent
-// loads would stand at the end of every row otherwise).
+// loads would stand at the end of every row otherwise).  With kLoss also sum_j e_j ((t_j - max t) - (z_j - z_max)), of which
+// the loss is made.
 struct Teacher {
-  float m;
-  double s;
+  float m, e;  // maximum; the own slot's exponential
+  double s, cross;
   bool any;
 };
-template <typename T, int L>
-__device__ __forceinline__ Teacher row_teacher(const DistillParams& P, int64_t row, const Slot& own) {
-  constexpr const T* kNoLogits = nullptr;
+template <typename T, int L, bool kLoss>
+__device__ __forceinline__ Teacher row_teacher(const DistillParams& P, int64_t row, const T* __restrict__ z, const Slot& own,
+                                               float z_max) {
   const int lane = threadIdx.x % L;
   float m = -__builtin_inff();
   bool any = false, bad = false;
   Slot at = own;
   for (int j = lane; j < P.top; j += L) {
-    if (j != lane) at = slot_at<T>(P, row, kNoLogits, j);
+    if (j != lane) at = slot_at<T>(P, row, static_cast<const T*>(nullptr), j);
     if (at.cls == -1) continue;
     bad |= at.cls == -2 || at.t != at.t;
     any |= at.t != -__builtin_inff();
@@ -197,36 +193,33 @@ __device__ __forceinline__ Teacher row_teacher(const DistillParams& P, int64_t r
   m = reduce_lanes<L, OpMax>(m);
   bad = any_lane<L>(bad);
   any = any_lane<L>(any) || bad;
-  double s = 0.0;
+  Teacher r{m, 0.0f, 0.0, 0.0, any};
   at = own;
   for (int j = lane; j < P.top; j += L) {
-    if (j != lane) at = slot_at<T>(P, row, kNoLogits, j);
-    if (at.cls != -1) s += (double)exp_slot(at.t, m, P.scale64);
+    if (j != lane) at = slot_at<T>(P, row, kLoss ? z : nullptr, j);
+    if (at.cls == -1) continue;
+    const float e = exp_slot(at.t, m, P.scale64);
+    if (j == lane) r.e = e;
+    r.s += (double)e;
+    if (kLoss && e != 0.0f)
+      r.cross = __builtin_fma((double)e, ((double)at.t - (double)m) - ((double)at.z - (double)z_max), r.cross);
   }
-  s = sum_lanes<L>(s);
-  return {m, bad ? __builtin_nan("") : s, any};
+  r.s = bad ? __builtin_nan("") : sum_lanes<L>(r.s);
+  if (kLoss) r.cross = sum_lanes<L>(r.cross);
+  return r;
 }
 
 // Loss of a row from its softmax statistics, by L lanes; keeps the statistics and, without a reduction, stores the loss.
+//   sum_j p_j (log p_j - log q_j) = sum_j p_j ((t_j - max t) - (z_j - max z)) / T + log(sum exp z / sum exp t)
 template <typename T, int L>
 __device__ __forceinline__ double row_loss(const DistillParams& P, int64_t row, const T* __restrict__ z, const Slot& own, float m,
                                            float s, bool store, bool& taught) {
-  const int lane = threadIdx.x % L;
-  const Teacher teacher = row_teacher<T, L>(P, row, own);
+  const Teacher teacher = row_teacher<T, L, true>(P, row, z, own, m);
   taught = teacher.any;
-  double loss = 0.0;
-  const double inv_t = 1.0 / P.temperature, inv_ps = 1.0 / teacher.s;
-  const double log_ratio = log((double)s * inv_ps);  // log p - log q = (t - max t) / T - (z - max z) / T + this
-  Slot at = own;
-  for (int j = lane; j < P.top; j += L) {
-    if (j != lane) at = slot_at<T>(P, row, z, j);
-    if (at.cls == -1 || !teacher.any) continue;
-    const double p = (double)exp_slot(at.t, teacher.m, P.scale64) * inv_ps;  // (NaN where a class is missing)
-    const double d = (((double)at.t - (double)teacher.m) - ((double)at.z - (double)m)) * inv_t + log_ratio;
-    if (p != 0.0) loss += p * d;
-  }
-  loss = sum_lanes<L>(loss) * P.temperature * P.temperature;
-  if (lane == 0 && store) {
+  const double inv_s = 1.0 / teacher.s;
+  const double loss =
+      teacher.any ? (teacher.cross * inv_s * P.inv_t + log((double)s * inv_s)) * P.temperature * P.temperature : 0.0;
+  if (threadIdx.x % L == 0 && store) {
     if (P.stats) {
       P.stats[2 * row] = m;
       P.stats[2 * row + 1] = s;
@@ -384,12 +377,12 @@ template <typename T, int L>
 __device__ __forceinline__ int row_shares(const DistillParams& P, int64_t row, int* cls, float* share) {
   constexpr const T* kNoLogits = nullptr;
   Slot at = slot_at<T>(P, row, kNoLogits, threadIdx.x % L);
-  const Teacher teacher = row_teacher<T, L>(P, row, at);
+  const Teacher teacher = row_teacher<T, L, false>(P, row, kNoLogits, at, 0.0f);
   const float inv_s = (float)(1.0 / teacher.s);
   for (int j = threadIdx.x % L; j < P.top; j += L) {
     if (j >= L) at = slot_at<T>(P, row, kNoLogits, j);
     cls[j] = at.cls;
-    share[j] = at.cls == -1 ? 0.0f : exp_slot(at.t, teacher.m, P.scale64) * inv_s;
+    share[j] = at.cls == -1 ? 0.0f : (j < L ? teacher.e : exp_slot(at.t, teacher.m, P.scale64)) * inv_s;
   }
   return !teacher.any ? 0 : teacher.s != teacher.s ? 2 : 1;
 }
@@ -605,7 +598,7 @@ void fill_common(DistillParams& P, const void* logits, int64_t stride, int64_t r
                  int teacher_dtype, const void* index, int index_bytes, int top, double temperature, int reduction) {
   P.z = logits; P.stride = stride; P.rows = rows; P.cols = cols; P.t = teacher; P.t_dtype = teacher_dtype;
   P.index = index; P.index64 = index_bytes == 8; P.top = top; P.temperature = temperature;
-  P.scale64 = kLog2e / temperature; P.scale = (float)P.scale64; P.reduction = reduction;
+  P.scale64 = kLog2e / temperature; P.inv_t = 1.0 / temperature; P.scale = (float)P.scale64; P.reduction = reduction;
 }
 
 }  // namespace

@@ -93,29 +93,10 @@ __device__ __forceinline__ double exp64(double x) {
 }
 #undef UR_CONSTANT
 
-// Steps of a reduction over the wave as in reduce_lanes: what each lane gets to combine its value with.
-template <int kStep>
-__device__ __forceinline__ uint32_t wave_other(uint32_t v) {
-  if constexpr (kStep < 4) {
-    constexpr int kCtrl[4] = {kDppXor1, kDppXor2, kDppHalfMirror, kDppMirror};
-    return dpp32<kCtrl[kStep]>(v);
-  } else {
-    const auto r = kStep == 4 ? __builtin_amdgcn_permlane16_swap(v, v, false, false)
-                              : __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return r[0] ^ r[1] ^ v;  // (one of the two is the lane's own)
-  }
-}
-template <int kStep = 0>
-__device__ __forceinline__ double wave_sum(double v) {
-  const uint64_t b = (uint64_t)__double_as_longlong(v);
-  const uint64_t o = ((uint64_t)wave_other<kStep>((uint32_t)(b >> 32)) << 32) | wave_other<kStep>((uint32_t)b);
-  v += __longlong_as_double((long long)o);
-  if constexpr (kStep < 5) v = wave_sum<kStep + 1>(v);
-  return v;
-}
+// the largest of the wave's numbers, in every lane
 template <int kStep = 0>
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-  v = max(v, wave_other<kStep>(v));
+  v = max(v, other_lane<kStep>(v));
   if constexpr (kStep < 5) v = wave_max<kStep + 1>(v);
   return v;
 }
@@ -135,7 +116,7 @@ __device__ int choose_wide(const RouteParams& P, const T* __restrict__ row, uint
     m = mf == -__builtin_inff() ? 0.0 : (double)mf;
     z = 0.0;
     for (int e = lane; e < E; e += 64) z += exp64((double)(float)row[e] - m);
-    z = wave_sum(z);
+    z = sum_lanes<64>(z);
   }
   // key of a candidate's c (by_score: of s where c would be the bare logit), 0 where it is not eligible
   const auto key = [&](int e, bool by_score) -> uint64_t {

@@ -96,6 +96,34 @@ __device__ __forceinline__ float reduce_lanes(float v) {
   return v;
 }
 
+// What step kStep (lanes 1, 2, 4, 8, 16, 32 apart, or the mirror that stands in for it) of such a reduction combines a lane's
+// value with.
+template <int kStep>
+__device__ __forceinline__ uint32_t other_lane(uint32_t v) {
+  if constexpr (kStep < 4) {
+    constexpr int kCtrl[4] = {kDppXor1, kDppXor2, kDppHalfMirror, kDppMirror};
+    return dpp32<kCtrl[kStep]>(v);
+  } else if constexpr (kStep == 4) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return r[0] ^ r[1] ^ v;  // (one of the two is the lane's own)
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return r[0] ^ r[1] ^ v;
+  }
+}
+
+// sum of 64-bit numbers over L consecutive lanes
+template <int L, int kStep = 0>
+__device__ __forceinline__ double sum_lanes(double v) {
+  if constexpr ((1 << kStep) < L) {
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    const uint64_t o = ((uint64_t)other_lane<kStep>((uint32_t)(b >> 32)) << 32) | other_lane<kStep>((uint32_t)b);
+    return sum_lanes<L, kStep + 1>(v + __longlong_as_double((long long)o));
+  } else {
+    return v;
+  }
+}
+
 // Sums over TPR threads: a group of lanes (TPR <= 64), or the whole workgroup through LDS (`part`: kN floats per
 // wave; the partial sums are added in wave order, so the result does not depend on timing).  The caller puts a barrier
 // between two uses of the same `part`.
