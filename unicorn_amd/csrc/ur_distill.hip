@@ -237,7 +237,8 @@ __device__ __forceinline__ void reduced_loss(const DistillParams& P, double sum,
   if (P.stats) P.stats[2 * P.rows] = (float)factor;
 }
 
-// Forward, L lanes a row (a row of few classes), kThreads / L rows a workgroup.
+// Forward, L lanes a row (a row of few classes), kThreads / L rows a workgroup.  100000 x 6 fp32 13 us, 30000 x 128 bf16 10.4,
+// 32768 x 1000 bf16 33 us (2.0 TB/s; 21 without the teacher's part): bound by the teacher's 64-bit arithmetic, once a wave.
 template <typename T, int L>
 __global__ void __launch_bounds__(kThreads) k_distill_fwd_rows(const DistillParams P) {
   constexpr int R = kThreads / L;
@@ -298,7 +299,8 @@ __device__ __forceinline__ void finish_row(const DistillParams& P, int64_t row, 
   }
 }
 
-// Forward, one workgroup a row.
+// Forward, one workgroup a row.  8192 x 32768 bf16 101 us (5.3 TB/s; 512 and 1024 threads 113 and 180), 4096 x 8101 fp16
+// 17.8 us (3.7 TB/s: one exponential and six other instructions an element, and the teacher at each row's end).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_distill_fwd(const DistillParams P) {
   __shared__ float part[2][kThreads / 64];
@@ -314,6 +316,7 @@ __global__ void __launch_bounds__(kThreads) k_distill_fwd(const DistillParams P)
 }
 
 // Forward, too few rows to fill the chip: a row is split over workgroups, whose maxima and sums a second launch merges.
+// 3 x 131071 bf16: 3.1 + 3.7 us, two latencies; one workgroup a row took 29.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_distill_split(const DistillParams P) {
   __shared__ float part[2][kThreads / 64];
@@ -482,7 +485,8 @@ __global__ void __launch_bounds__(kThreads) k_distill_bwd_rows(const DistillPara
   if (mine) write_shares<T>(P, r, z, out, cls[sub], share[sub], 0, P.cols, t, L);
 }
 
-// a workgroup takes one row or (gridDim.x > 1) a part of one
+// A workgroup takes one row or (P.splits > 1) a part of one.  8192 x 32768 bf16 210 us (5.1 TB/s; with ordinary stores 250),
+// 4096 x 8101 fp16 31.5 us (4.2), 3 x 131071 bf16 10.3 us.
 template <typename T, int TH>
 __global__ void __launch_bounds__(TH) k_distill_bwd(const DistillParams P) {
   __shared__ int cls[kMaxTop];

@@ -687,7 +687,8 @@ __global__ void __launch_bounds__(kThreads, resident(sizeof(T), LPR, IPL)) k_rou
   for (int e = threadIdx.x; e < E; e += kThreads) out[e] = hist[e];
 }
 
-// counts = the sums of the workgroups' counts: 32 candidates a workgroup, 32 groups of threads over the partial rows
+// counts = the sums of the workgroups' counts: 32 candidates a workgroup, 32 groups of threads over the partial rows (1024 of
+// them: 4.6 us, the latency of 32 loads and of the sums after them; 257: 1.9 us).  Nothing has to be cleared beforehand.
 __global__ void __launch_bounds__(1024) k_route_counts(const RouteParams P) {
   __shared__ int acc[32][33];
   const int c = threadIdx.x & 31, grp = threadIdx.x >> 5, e = blockIdx.x * 32 + c;
@@ -709,7 +710,8 @@ __global__ void __launch_bounds__(1024) k_route_counts(const RouteParams P) {
 //     and nothing cancels where one choice has nearly all the weight;
 //     softmax: dl_j = scale share_j d_j for the chosen, exactly 0 for all others; sigmoid: times (1 - s_j)
 //   not renormalised: sigmoid: dl_j = scale dw_j s_j (1 - s_j); softmax: dl_e = s_e (ds_e - sum_j ds_j s_j), every candidate
-// A row of gradients is put together in LDS (zeros and the k chosen) and stored in 16-byte pieces.
+// A row of gradients is put together in LDS (zeros and the k chosen) and stored in 16-byte pieces: 131072 x 256 bf16, top 8,
+// 21 to 24 us, bound by its 67 MB of stores.
 template <typename T, int LPR>
 __global__ void __launch_bounds__(kThreads) k_route_bwd(const RouteParams P) {
   constexpr int R = 64 / LPR, kRow = LPR * 16, N = Elem<T>::kN;
