@@ -241,16 +241,23 @@ __device__ __forceinline__ void row_softmax(const T* __restrict__ row, int E, in
 // largest candidate; the few candidates that reach it (about 10 of 256) go to a list in LDS as (key, index) and each finds
 // its rank by counting the larger ones.
 
-// how many of the values that a row's other 15 lanes hold (two a lane) are >= v, >= w
-template <int kRor>
-__device__ __forceinline__ void count_ge16(float v, float w, int& nv, int& nw) {
-  if constexpr (kRor > 0) {
-    const float a = __uint_as_float(dpp32<0x120 + kRor>(__float_as_uint(v)));
-    const float b = __uint_as_float(dpp32<0x120 + kRor>(__float_as_uint(w)));
-    nv += (a >= v) + (b >= v);
-    nw += (a >= w) + (b >= w);
-    count_ge16<kRor - 1>(v, w, nv, nw);
-  }
+// the number that the lane kXor away holds, inside 16 lanes
+template <int kXor>
+__device__ __forceinline__ float across(float v) {
+  if constexpr (kXor == 4) return across<7>(across<3>(v));
+  constexpr int kCtrl = kXor == 1 ? kDppXor1 : kXor == 2 ? kDppXor2 : kXor == 3 ? 0x1B : kXor == 7 ? kDppHalfMirror
+                      : kXor == 8 ? 0x128 : kDppMirror;
+  return __uint_as_float(dpp32<kCtrl>(__float_as_uint(v)));
+}
+// A step of a sorting network over 16 lanes, largest first: of each pair of lanes the lower takes the larger number.  `way`: +inf
+// in the lower lane, -inf in the other, which makes the median of three a maximum or a minimum without a comparison.
+template <int kXor>
+__device__ __forceinline__ float sort_step(float v, float way) { return __builtin_amdgcn_fmed3f(v, across<kXor>(v), way); }
+__device__ __forceinline__ float sort16(float v, const float (&way)[4]) {
+  v = sort_step<1>(v, way[0]);
+  v = sort_step<1>(sort_step<3>(v, way[1]), way[0]);
+  v = sort_step<1>(sort_step<2>(sort_step<7>(v, way[2]), way[1]), way[0]);
+  return sort_step<1>(sort_step<2>(sort_step<4>(sort_step<15>(v, way[3]), way[2]), way[1]), way[0]);
 }
 
 // lane i of this lane's row of LPR (i the same in the whole wave)
@@ -274,7 +281,7 @@ __device__ __forceinline__ float max_rows(float v) {
   return v;
 }
 
-// A lower bound (at least the lowest finite number) of the (k+1)-th largest value, from the maxima of two sets of values a
+// A finite lower bound (or the lowest finite number) of the (k+1)-th largest value, from the maxima of two sets of values a
 // lane.  (Two, because groups that were not taken leave lanes empty: with half of 16 lanes left, their 16 sets still bound
 // the 9th largest.)
 template <int LPR>
@@ -284,9 +291,14 @@ __device__ __forceinline__ float prune_bound(float v, float w, int k) {
   if (LPR == 16 || (LPR > 16 && k + 1 <= 8)) {  // 32 sets: lanes 16, 32, 48 apart are put together
     v = max_rows<LPR>(v);
     w = max_rows<LPR>(w);
-    int nv = 1 + (w >= v), nw = 1 + (v >= w);
-    count_ge16<15>(v, w, nv, nw);
-    bound = reduce_lanes<16, OpMax>(__builtin_fmaxf(nv >= k + 1 ? v : -kInf, nw >= k + 1 ? w : -kInf));
+    const int t = threadIdx.x & 15;
+    float way[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) way[i] = (t >> i) & 1 ? -kInf : kInf;
+    // the 16 largest of both, in an order that four more steps sort; the (k+1)-th largest is lane k's
+    v = __builtin_fmaxf(sort16(v, way), across<15>(sort16(w, way)));
+    v = sort_step<1>(sort_step<2>(sort_step<4>(sort_step<8>(v, way[3]), way[2]), way[1]), way[0]);
+    bound = reduce_lanes<16, OpMax>(t >= k ? v : -kInf);
   } else {
     int nv = 0, nw = 0;
     for (int i = 0; i < LPR; ++i) {
@@ -296,7 +308,7 @@ __device__ __forceinline__ float prune_bound(float v, float w, int k) {
     }
     bound = reduce_lanes<LPR, OpMax>(__builtin_fmaxf(nv >= k + 1 ? v : -kInf, nw >= k + 1 ? w : -kInf));
   }
-  return __builtin_fmaxf(bound, -__FLT_MAX__);
+  return __builtin_fminf(__builtin_fmaxf(bound, -__FLT_MAX__), __FLT_MAX__);
 }
 
 // sum of the lanes before this one, inside groups of LPR lanes (row shifts by DPP, then whole rows of 16)
@@ -567,10 +579,13 @@ __global__ void __launch_bounds__(kThreads, resident(sizeof(T), LPR, IPL)) k_rou
         }
         bound = prune_bound<LPR>(in_group ? v : -kInf, in_group ? w : -kInf, k);
       }
-      uint32_t reach = 0;
+      // by the signs of the differences: no comparison, no carry to wait for.  A bound of 0 is made -0, from which neither 0 nor
+      // -0 leaves -0.
+      if (bound == 0.0f) bound = -0.0f;
+      uint32_t below = 0;
 #pragma unroll
-      for (int i = IPL - 1; i >= 0; --i) reach = 2 * reach + (c[i] >= bound);
-      if (!in_group) reach = 0;
+      for (int i = IPL - 1; i >= 0; --i) below = __builtin_amdgcn_alignbit(below, __float_as_uint(c[i] - bound), 31);
+      uint32_t reach = in_group ? ~below & ((1u << IPL) - 1) : 0;
       wave_lds_handoff();
 #pragma unroll
       for (int i = 0; i < IPL; ++i) vals[first + i] = c[i];

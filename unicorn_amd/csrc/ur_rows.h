@@ -63,7 +63,7 @@ __device__ __forceinline__ void store_from_float(void* p, int dtype, int64_t i, 
 // for the exchange of two halves because the halves are uniform by then.  Beyond, the two row-swap instructions.
 template <int kCtrl>
 __device__ __forceinline__ uint32_t dpp32(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, kCtrl, 0xf, 0xf, false);
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kCtrl, 0xf, 0xf, true);  // (every lane has a source: nothing is left as it was)
 }
 constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E, kDppHalfMirror = 0x141, kDppMirror = 0x140;
 
