@@ -99,7 +99,8 @@ __device__ __forceinline__ void load_params(const void* p, int dtype, int64_t at
 
 // ---- rows that fit the registers of TPR threads, NV 16-byte vectors each -------------------------------------------
 // Forward: 65536 x 1024 bf16 50 us (5.4 TB/s), 8192 x 4096 fp32 50 us (5.3), 6151 x 1926 fp16 of stride 1961 12.4 us (3.8: rows
-// that start anywhere, and a short launch); 192 x 512 fp32 3.2 us, the latency of one row.
+// that start anywhere, and a short launch); 192 x 512 fp32 3.2 us, the latency of one row.  Rows that take a whole workgroup of
+// 1024 threads are stored past the caches (2000 x 20000 fp32 77 us against 89; shorter rows lose: 65536 x 1024 bf16 51 against 49).
 template <typename T, int TPR, int NV>
 __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR) k_ln_fwd(const LnParams P) {
   constexpr int N = Elem<T>::kN, kRows = TPR <= 64 ? 256 / TPR : 1;
@@ -149,7 +150,8 @@ __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR) k_ln_fwd(const LnParams
     typename Elem<T>::Vec o;
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] = (T)__builtin_fmaf(((float)v[i][j] - mean) * rstd, w[j], b[j]);
-    store_span<T>(y, at.at, o);
+    if constexpr (TPR == 1024) store16_past<T>(y, at.at, P.cols, o);
+    else store_span<T>(y, at.at, o);
   }
 }
 
@@ -423,8 +425,9 @@ __global__ void __launch_bounds__(1024) k_ln_param_sums(const LnParams P) {
 
 // ---- long rows: a row is split over workgroups ----------------------------------------------------------------------
 // Forward: (1) every chunk's mean and sum of squared differences from it, (2) each chunk's workgroup merges the row's
-// chunks and writes its part.  x is read twice, the second time mostly from the caches: 129 x 65536 fp32 6 + 12.5 us (34 MB
-// each way; one workgroup a row, with 64 elements a thread, took 25).
+// chunks and writes its part.  x is read twice, the second time mostly from the caches, which the results' stores leave alone:
+// 129 x 65536 fp32 5.5 + 11 us (34 MB each way; with ordinary stores 6 + 12.5; one workgroup a row, with 64 elements a thread,
+// took 25).
 constexpr int kLongThreads = 256, kLongVecs = 4;
 
 // parameters of columns col ..., as far as they lie inside the row
@@ -512,13 +515,13 @@ __global__ void __launch_bounds__(kLongThreads) k_ln_long_apply(const LnParams P
     typename Elem<T>::Vec o;
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] = (T)__builtin_fmaf(((float)v[j] - mean) * rstd, w[j], b[j]);
-    store16<T>(y, col, c1, o);
+    store16_past<T>(y, col, c1, o);
   }
 }
 
 // Backward: (1) every chunk's sums of g and g h, (2) a workgroup takes a strip of columns through a range of rows: dx, and
-// its columns' partial weight sums; (3) k_ln_param_sums.  x and dy are read twice: 1024 x 32768 bf16 82 us in all, 65 of them
-// without the weights' gradients; 129 x 65536 fp32 37 us.
+// its columns' partial weight sums; (3) k_ln_param_sums.  x and dy are read twice: 1024 x 32768 bf16 77 us in all, 60 of them
+// without the weights' gradients (82 and 65 with ordinary stores); 129 x 65536 fp32 36 us.
 template <typename T>
 __global__ void __launch_bounds__(kLongThreads) k_ln_long_bwd_sums(const LnParams P) {
   constexpr int N = Elem<T>::kN;
@@ -590,7 +593,7 @@ __global__ void __launch_bounds__(kLongThreads) k_ln_long_bwd_apply(const LnPara
       ab[j] += d;
       o[j] = (T)(now.rstd * (d * w[j] - c1 - h * c2));
     }
-    if (P.y && inside) store16<T>(static_cast<T*>(P.y) + row * P.cols, col, P.cols, o);
+    if (P.y && inside) store16_past<T>(static_cast<T*>(P.y) + row * P.cols, col, P.cols, o);
     now = next;
   }
   if (P.parts == 0 || !inside) return;

@@ -24,7 +24,7 @@ typedef float f32x4_lds __attribute__((ext_vector_type(4)));
 // Workgroups of the forward a CU, as many as are resident at once (of four waves, one on each SIMD): four of at most 128
 // registers; three for 16 candidates of fp32 a lane and, for LDS, for the longest rows.  One round of them and no more: a
 // second, short round lasts as long as a full one (131072 x 256 with 768 resident: 1024 workgroups 104 us, 768 workgroups 87).
-// Five or six of fewer registers gain nothing (131072 x 64: 40 against 39 us): the forward is bound by instruction issue.
+// Five or six of fewer registers gain nothing (131072 x 64: 39 against 40 us): the forward is bound by instruction issue.
 constexpr int kCus = 256;
 constexpr int resident(int item_bytes, int lpr, int ipl) { return ipl == 16 && (lpr == 64 || item_bytes == 4) ? 3 : 4; }
 
@@ -233,9 +233,9 @@ __device__ __forceinline__ void row_softmax(const T* __restrict__ row, int E, in
 // same (logit, bias) twice.  Without a bias the logits themselves are compared and nothing has to be redone.  Such rows are
 // noted and done after every kSteps rounds, outside the loop over rows, which has the registers to itself then.
 //
-// Bound by instruction issue, not by memory: 131072 rows of 256 bf16, sigmoid with bias and 4 of 8 groups, top 8: 75 us (67 MB
-// read: 0.9 TB/s), softmax without a bias 44 us; 4099 x 64: 11 us, most of it the latency of one row after the other that is
-// done in 64 bits.  All logits equal (every row is done in 64 bits): 567 us.
+// Bound by instruction issue, not by memory: 131072 rows of 256 bf16, sigmoid with bias and 4 of 8 groups, top 8: 66 us (67 MB
+// read: 1 TB/s; 54 without the 64-bit choice), softmax without a bias 36 us; 4099 x 64: 7 us, half of it the latency of a
+// row that is done in 64 bits.  All logits equal (every row is done in 64 bits): 550 us.
 //
 // The top-k is not taken by k rounds of a maximum: the (k+1)-th largest of the lanes' maxima is a lower bound of the (k+1)-th
 // largest candidate; the few candidates that reach it (about 10 of 256) go to a list in LDS as (key, index) and each finds
@@ -281,6 +281,7 @@ __device__ __forceinline__ float max_rows(float v) {
   return v;
 }
 
+// (131072 x 256: 68 us; with the maxima ranked by comparing each with all others 75.)
 // A finite lower bound (or the lowest finite number) of the (k+1)-th largest value, from the maxima of two sets of values a
 // lane.  (Two, because groups that were not taken leave lanes empty: with half of 16 lanes left, their 16 sets still bound
 // the 9th largest.)

@@ -45,6 +45,13 @@ __device__ __forceinline__ void store16(T* __restrict__ row, int64_t col, int64_
     if (col + j < cols) row[col + j] = v[j];
 }
 
+// the same for a result that nobody reads soon, past the caches, which keep something better
+template <typename T>
+__device__ __forceinline__ void store16_past(T* __restrict__ row, int64_t col, int64_t cols, typename Elem<T>::Vec v) {
+  if (col + Elem<T>::kN <= cols) __builtin_nontemporal_store(v, reinterpret_cast<typename Elem<T>::Vec*>(row + col));
+  else store16<T>(row, col, cols, v);
+}
+
 // one element of a tensor whose type is known at run time only (parameters, small side inputs)
 __device__ __forceinline__ float load_as_float(const void* p, int dtype, int64_t i) {
   if (dtype == UR_F32) return static_cast<const float*>(p)[i];
