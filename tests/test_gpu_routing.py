@@ -431,3 +431,19 @@ def test_more_rows_than_a_launch_holds_threads_for():
         grads.append(torch.autograd.grad(r.weights, t, torch.ones((), device="cuda").expand_as(r.weights))[0])
     assert r.counts.sum().item() == len(x)
     assert bool((grads[1].view(-1, 8192) == grads[0].view(1, 8192)).all())
+
+
+@pytest.mark.parametrize("cands,k,times", [(8, 3, 5000), (64, 6, 2500), (300, 5, 1100), (600, 9, 480)])
+def test_many_rows_that_float32_cannot_order(cands, k, times):
+    """scores of 1 - 1e-6 and closer: nearly every row is chosen in 64 bits, in workgroups that take many rows one after the
+    other; the same rows over and over give the same"""
+    from unicorn_amd.routing import route_candidates
+    g = torch.Generator(device="cuda").manual_seed(cands)
+    part = (14.0 + 3.0 * torch.randn(256, cands, generator=g, device="cuda")).half()
+    bias = 1e-6 * torch.randn(cands, generator=g, device="cuda")
+    kw = dict(bias=bias, score="sigmoid", groups=4, top_groups=2, group_score="max")
+    check_all(part, k, **kw)
+    small, large = route_candidates(part, k, **kw), route_candidates(part.repeat(times, 1), k, **kw)
+    assert bool((large.indices.view(times, -1) == small.indices.view(1, -1)).all())
+    assert bool((large.weights.view(times, -1) == small.weights.view(1, -1)).all())
+    assert torch.equal(large.counts, small.counts * times)
