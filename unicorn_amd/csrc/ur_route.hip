@@ -229,9 +229,10 @@ __device__ __forceinline__ void row_softmax(const T* __restrict__ row, int E, in
 
 // ---- forward: LPR lanes a row, IPL consecutive candidates a lane -----------------------------------------------------
 // The choice is made in fp32 and redone in 64 bits (choose_wide) for the rows where fp32 cannot tell: with a bias, when two
-// neighbours of the order -- or the last group taken and the first one left -- are closer than fp32's error and are not the
-// same (logit, bias) twice.  Without a bias the logits themselves are compared and nothing has to be redone.  Such rows are
-// noted and done after every kSteps rounds, outside the loop over rows, which has the registers to itself then.
+// neighbours of the order -- the last one taken and any candidate left among them, or the last group taken and the first one
+// left -- are closer than fp32's error and are not the same (logit, bias) twice.  Without a bias the logits themselves are compared
+// and nothing has to be redone.  Such rows are noted and done after every kSteps rounds, outside the loop over rows, which
+// has the registers to itself then.
 //
 // Bound by instruction issue, not by memory: 131072 rows of 256 bf16, sigmoid with bias and 4 of 8 groups, top 8: 66 us (67 MB
 // read: 1 TB/s; 54 without the 64-bit choice), softmax without a bias 36 us; 4099 x 64: 7 us, half of it the latency of a
@@ -656,12 +657,31 @@ __global__ void __launch_bounds__(kThreads, resident(sizeof(T), LPR, IPL)) k_rou
 
       const uint64_t got = t < k ? slots[t] : 0;
       const int at = got ? kMaxCands - (int)(uint32_t)got : -1;
+      // Neighbours of the order that fp32 cannot tell, unless they are one (logit, bias) twice.  Where the last one taken and the
+      // first one left are one pair, this pair says nothing of what comes behind it: every candidate is looked at, also those
+      // that the bound or the cut of equal values kept off the list.  (Larger values are in slots before, where each has been held
+      // against its neighbour.)
+      const float slot_value = key_value((uint32_t)(got >> 32));
+      bool cut_same = false;
       if (P.bias && got) {
         const uint64_t next = slots[t + 1];
-        const float v = key_value((uint32_t)(got >> 32)), v2 = key_value((uint32_t)(next >> 32));
+        const float v = slot_value, v2 = key_value((uint32_t)(next >> 32));
         if (next && v - v2 <= err + 0x1p-22f * (fabsf(v) + fabsf(v2))) {
           const int at2 = kMaxCands - (int)(uint32_t)next;
-          close |= !((float)src[at] == (float)src[at2] && P.bias[at] == P.bias[at2]);
+          const bool same = (float)src[at] == (float)src[at2] && P.bias[at] == P.bias[at2];
+          close |= !same;
+          cut_same = same && t == k - 1;
+        }
+      }
+      if (__any(cut_same)) {
+        const float worst = __shfl(slot_value, k - 1, LPR);
+        const int at_cut = __shfl(cut_same ? at : -1, k - 1, LPR);
+        if (at_cut >= 0 && in_group) {
+          const float l_cut = (float)src[at_cut], b_cut = P.bias[at_cut];
+#pragma unroll
+          for (int i = 0; i < IPL; ++i)
+            if (c[i] != -kInf && c[i] <= worst && worst - c[i] <= err + 0x1p-22f * (fabsf(worst) + fabsf(c[i])))
+              close |= !((float)src[first + i] == l_cut && bias[i] == b_cut);
         }
       }
       const uint64_t all_close = __ballot(close && mine);
