@@ -328,7 +328,7 @@ int ur_layer_norm_backward(const void* grad_y, int64_t grad_row_stride, const vo
  *   groups: consecutive runs of cands / groups candidates; a group's value is its largest c or the sum of its two largest;
  *   the `top_groups` best groups stay ; indices = the top_k largest c left, largest first ; ties: the lowest index ;
  *   weights = scale * s / (sum of the chosen s) (renormalize != 0) or scale * s.
- *   The order is that of the 64-bit values of c.  A candidate with l = -inf or bias = -inf is not eligible; a slot that no
+ *   The order is that of the 64-bit values of c.  A candidate with l = -inf or bias = -inf is not eligible, whatever the other is; a slot that no
  *   eligible candidate is left for holds index -1 and weight 0.  NaN counts as +inf and makes weights NaN.
  *   logits (rows, cands), row i at logits + i * row_stride ; weights fp32, indices int64 (rows, top_k) ; counts int32 (cands).
  *   At most 1024 candidates, 64 choices, 64 groups (UR_ERR_UNSUPPORTED beyond).

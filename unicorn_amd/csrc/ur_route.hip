@@ -121,7 +121,7 @@ __device__ int choose_wide(const RouteParams& P, const T* __restrict__ row, uint
   // key of a candidate's c (by_score: of s where c would be the bare logit), 0 where it is not eligible
   const auto key = [&](int e, bool by_score) -> uint64_t {
     const double l = (double)(float)row[e];
-    if (l == -inf) return 0;
+    if (l == -inf || (P.bias && P.bias[e] == -__builtin_inff())) return 0;
     if (!P.bias && !by_score) return order_key(l);
     const double s = P.sigmoid ? 1.0 / (1.0 + exp64(-l)) : exp64(l - m) / z;
     const double c = P.bias ? s + (double)P.bias[e] : s;
@@ -470,9 +470,9 @@ __global__ void __launch_bounds__(kThreads, resident(sizeof(T), LPR, IPL)) k_rou
         if (P.bias) {
 #pragma unroll
           for (int i = 0; i < IPL; ++i) s[i] += bias[i];
-          if (odd) {
+          if (odd) {  // (a NaN score does not take a ruling out back)
 #pragma unroll
-            for (int i = 0; i < IPL; ++i) s[i] = c[i] == -kInf ? -kInf : s[i];
+            for (int i = 0; i < IPL; ++i) s[i] = c[i] == -kInf || bias[i] == -kInf ? -kInf : s[i];
           }
 #pragma unroll
           for (int i = 0; i < IPL; ++i) c[i] = s[i];

@@ -13,7 +13,7 @@ tell are still ordered as in 64 bits; without a bias the logits are compared.
 
 weights: s of the chosen, divided by their sum when `renormalize`, times `scale`; float32, largest c first, with a gradient
 to the logits.  indices: int64; counts: int32, how many rows took each candidate.  A logit of -inf (or a bias of -inf) rules
-a candidate out; a slot that nothing is left for holds index -1 and weight 0, and adds nothing to the gradient.  NaN
+a candidate out, whatever the other is; a slot that nothing is left for holds index -1 and weight 0, and adds nothing to the gradient.  NaN
 counts as +inf; with "softmax" a NaN or an infinite logit makes all weights of its row NaN, with "sigmoid" a NaN that
 is chosen does.
 """
