@@ -9,6 +9,7 @@
 // loaded: its entry points are passed in by address (bind).
 #include <torch/extension.h>
 
+#include <ATen/TensorSubclassLikeUtils.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -16,6 +17,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <map>
 #include <stdexcept>
@@ -115,11 +117,25 @@ void* ptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr
 const void* cptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 Tensor or_none(const std::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 
-// The nodes know nothing of forward-mode differentiation: a tangent would be dropped without a word.
-void no_tangent(std::initializer_list<Tensor> inputs) {
-  for (const Tensor& t : inputs)
-    if (t.defined() && t._fw_grad(0).defined())
-      throw std::runtime_error("forward-mode differentiation is not supported by this operator");
+// What the nodes know nothing of is refused.  A tangent of forward-mode differentiation would be dropped without a word.  A
+// tracer records the allocation of a result but not the kernel that fills it: the trace would return uninitialised memory.
+// Tensors of a function transform, and subclasses that dispatch for themselves, have no memory of their own to hand over.
+void plain_inputs(std::initializer_list<Tensor> inputs) {
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  bool traced = torch::jit::tracer::isTracing();
+  if (c10::impl::dispatch_mode_enabled())
+    for (const auto mode : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+      traced |= TorchDispatchModeTLS::get_mode(mode).has_value();
+  if (traced) throw std::runtime_error("tracing is not supported by this operator: its kernels would not be in the trace");
+  for (const Tensor& t : inputs) {
+    if (!t.defined()) continue;
+    const auto keys = t.key_set();
+    if (keys.has_any(at::kFunctorchWrappedTensors) || keys.has(c10::DispatchKey::Batched) || keys.has(c10::DispatchKey::Python))
+      throw std::runtime_error("function transforms (torch.func, batched gradients) and tensor subclasses with a dispatch of "
+                               "their own are not supported by this operator");
+    if (t._fw_grad(0).defined()) throw std::runtime_error("forward-mode differentiation is not supported by this operator");
+  }
 }
 
 // A leaf's gradient accumulator belongs to the stream of the graph that made it and lives as long as that graph.  A captured
@@ -208,6 +224,7 @@ struct LayerNormBackward : Node {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(3);
     if (!grads[0].defined()) return out;
+    plain_inputs({grads[0]});
     no_accumulator_of_default_stream(*this);
     const Tensor xs = x.unpack(), ws = weight.unpack();
     std::tie(out[0], out[1], out[2]) =
@@ -226,7 +243,7 @@ struct LayerNormBackward : Node {
 
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
   const Tensor w = or_none(weight), b = or_none(bias);
-  no_tangent({x, w, b});
+  plain_inputs({x, w, b});
   const bool record = compute_requires_grad(x, w, b);
   auto [y, stats] = layer_norm_forward(x, w, b, eps, record);
   if (record) {
@@ -290,6 +307,7 @@ struct RouteBackward : Node {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(1);
     if (!grads[0].defined()) return out;
+    plain_inputs({grads[0]});
     no_accumulator_of_default_stream(*this);
     out[0] = route_backward(grads[0], logits.unpack(), weights.unpack(shared_from_this()), indices.unpack(), score, renormalize,
                             scale);
@@ -307,7 +325,7 @@ struct RouteBackward : Node {
 std::tuple<Tensor, Tensor, Tensor> route(const Tensor& logits, const std::optional<Tensor>& bias, int64_t top_k, int64_t score,
                                          int64_t groups, int64_t top_groups, int64_t group_score, bool renormalize,
                                          double scale) {
-  no_tangent({logits});
+  plain_inputs({logits, or_none(bias)});
   auto out = route_forward(logits, bias, top_k, score, groups, top_groups, group_score, renormalize, scale);
   if (compute_requires_grad(logits)) {
     auto node = std::make_shared<RouteBackward>();
@@ -373,6 +391,7 @@ struct DistillBackward : Node {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(1);
     if (!grads[0].defined()) return out;
+    plain_inputs({grads[0]});
     no_accumulator_of_default_stream(*this);
     const Tensor z = logits.unpack();
     out[0] = distill_backward(grads[0], z, teacher.unpack(), index.unpack(), temperature, reduction, stats);
@@ -389,7 +408,7 @@ struct DistillBackward : Node {
 };
 
 Tensor distill(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature, int64_t reduction) {
-  no_tangent({logits});
+  plain_inputs({logits, teacher, index});
   const bool record = compute_requires_grad(logits);
   auto [loss, stats] = distill_forward(logits, teacher, index, temperature, reduction, record);
   if (record) {
