@@ -162,6 +162,10 @@ __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR) k_ln_fwd(const LnParams
 // 65536 x 1024 bf16 79 us + 4.7 for the sums (402 MB: 4.9 TB/s); with 512 workgroups 89.  8192 x 4096 fp32 82 us (4.9);
 // 2048 x 16384 bf16 66 us, of which 26 go into the partial sums (33 MB written and read again).
 constexpr int kBwdThreads = 1024, kBwdBlocks = 256;
+// A thread adds at most so many rows' terms in fp32 before its sum joins the others in 64 bits (k_ln_param_sums): an fp32 sum
+// loses up to half a step a term.  From 128 rounds of 256 workgroups on there are more workgroups than resident at once;
+// their partial rows are 1/32 of x at the most.
+constexpr int kSerialRows = 128;
 
 // a workgroup's sum of one column (which: 0 weight, 1 bias): to its partial row, or, from the only workgroup, to the result
 __device__ __forceinline__ void put_sum(const LnParams& P, int part, int which, int64_t col, float v) {
@@ -643,7 +647,7 @@ LnPlan ln_plan(int64_t rows, int64_t cols, int dtype, bool backward) {
     }
   if (p.tpr) {
     const int64_t groups = ceil_div(rows, kBwdThreads / p.tpr);
-    p.grid = (int)ceil_div(groups, ceil_div(groups, kBwdBlocks));  // (every workgroup as many rows)
+    p.grid = (int)ceil_div(groups, std::min<int64_t>(ceil_div(groups, kBwdBlocks), kSerialRows));  // (all as many rows)
     p.ws_parts = backward && p.grid > 1 ? (int64_t)p.grid * 2 * cols : 0;
     return p;
   }
@@ -654,8 +658,10 @@ LnPlan ln_plan(int64_t rows, int64_t cols, int dtype, bool backward) {
   p.chunks = (int)ceil_div(cols, p.chunk);
   p.ws_stats = rows * p.chunks * 2;
   const int64_t strips = ceil_div(cols, (int64_t)kLongThreads * n);
-  // row ranges: about 1024 workgroups, and at least 8 rows for the 2 D floats a range leaves behind
+  // row ranges: about 1024 workgroups, and 8 rows at least, kSerialRows at most, for the 2 D floats a range leaves behind (as far
+  // as the grid's second dimension goes: 8.4 million rows of more than 4096 vectors are not in memory)
   p.grid = (int)std::min<int64_t>(ceil_div(rows, 8), ceil_div(1024, strips));
+  p.grid = (int)std::max<int64_t>(p.grid, std::min<int64_t>(ceil_div(rows, kSerialRows), 65535));
   p.ws_parts = backward && p.grid > 1 ? (int64_t)p.grid * 2 * cols : 0;
   return p;
 }

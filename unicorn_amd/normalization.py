@@ -6,7 +6,8 @@ predict shape, texture and candidate poses (the reference's heads, unicorn.py:24
 
 x: float32, float16 or bfloat16, any shape and strides (rows with a dense last dimension and an even spacing are read where
 they lie, others are copied first); weight and bias have x's type or float32.  Statistics and sums are float32, the
-result is rounded once.  The gradients of weight and bias are summed in a fixed order: the same call gives the same bits.
+result is rounded once.  The gradients of weight and bias are summed in a fixed order, at most 128 rows one after the other in
+float32 and those sums in 64 bits: the same call gives the same bits.
 No rows give an empty result and zero parameter gradients.  A row that holds an infinity or a NaN becomes NaN.
 """
 import torch
