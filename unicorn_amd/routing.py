@@ -71,5 +71,6 @@ def route_candidates(logits, top_k, bias=None, score="softmax", groups=1, top_gr
 def update_balance_bias(bias, counts, rate):
     """In place: a candidate taken more often than the average loses `rate`, one taken less often gains it.  In a
     data-parallel job `counts` is summed over the ranks first."""
-    c = counts.to(torch.float32)
-    return bias.add_(torch.sign(c.mean() - c), alpha=float(rate))
+    c = counts.to(torch.float64 if counts.is_floating_point() else torch.int64)
+    # against the average without dividing: float32 cannot tell counts beyond 2^24 from one another
+    return bias.add_(torch.sign(torch.sub(c.sum(), c, alpha=c.numel())), alpha=float(rate))
