@@ -53,8 +53,12 @@ def chosen_poses(R, T, routing):
 
 def candidate_loss(errors, routing, scores, temperature=1.0, score_weight=1.0):
     """Per image (B,): the chosen candidates' errors (B, k) under the routing weights, plus `score_weight` times the
-    divergence of the scores from softmax(-errors / temperature) over the chosen candidates (empty slots left out).  Errors
-    get their gradient through the first term only."""
-    expected = (routing.weights * errors).sum(1)
+    divergence of the scores from softmax(-errors / temperature) over the chosen candidates (empty slots left out, whatever
+    their error).  Errors get their gradient through the first term only."""
+    if not temperature > 0.0:
+        raise ValueError(f"temperature must be positive, got {temperature}")
+    if errors.shape != routing.indices.shape:
+        raise ValueError(f"errors must have shape {tuple(routing.indices.shape)}, got {tuple(errors.shape)}")
+    expected = (routing.weights * torch.where(routing.indices < 0, 0.0, errors)).sum(1)  # (0 times a NaN would be NaN)
     teacher = (errors.detach() / -float(temperature)).to(torch.float32)
     return expected + score_weight * distill_top_logits(scores, teacher, routing.indices, reduction="none")
