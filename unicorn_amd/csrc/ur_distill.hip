@@ -226,7 +226,7 @@ __device__ __forceinline__ double row_loss(const DistillParams& P, int64_t row, 
     }
     if (P.reduction == UR_REDUCE_NONE) P.loss[row] = (float)loss;
   }
-  return (double)(float)loss;
+  return loss;  // (a reduction adds the rows in 64 bits and rounds once)
 }
 
 // the reduced loss from the sum of the rows' losses and the number of rows that have a teacher; keeps the factor for the
