@@ -432,11 +432,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bind", &bind, "hand over the addresses of the library's entry points, {name: address}");
   m.def("layer_norm", &layer_norm, guard());
   m.def("layer_norm_forward", &layer_norm_forward, guard());
-  m.def("layer_norm_backward", &layer_norm_backward, guard());
   m.def("route", &route, guard());
-  m.def("route_forward", &route_forward, guard());
-  m.def("route_backward", &route_backward, guard());
   m.def("distill", &distill, guard());
-  m.def("distill_forward", &distill_forward, guard());
-  m.def("distill_backward", &distill_backward, guard());
 }

@@ -635,7 +635,7 @@ NODES_PATH = os.path.join(_HERE, "lib", "unicorn_autograd.so")
 
 def nodes():
     """The C++ module of the operators' autograd nodes (csrc/ur_autograd.cpp), bound to the library loaded here: layer_norm,
-    route, distill, and each one's `_forward` / `_backward` without a graph.  Arguments are checked by the Python layer."""
+    route, distill, and layer_norm_forward without a graph.  Arguments are checked by the Python layer."""
     global _nodes
     if _nodes is None:
         if not os.path.exists(NODES_PATH):
