@@ -121,11 +121,11 @@ __device__ int choose_wide(const RouteParams& P, const T* __restrict__ row, uint
   // key of a candidate's c (by_score: of s where c would be the bare logit), 0 where it is not eligible
   const auto key = [&](int e, bool by_score) -> uint64_t {
     const double l = (double)(float)row[e];
-    if (l == -inf || (P.bias && P.bias[e] == -__builtin_inff())) return 0;
+    if (l == -inf) return 0;
     if (!P.bias && !by_score) return order_key(l);
     const double s = P.sigmoid ? 1.0 / (1.0 + exp64(-l)) : exp64(l - m) / z;
-    const double c = P.bias ? s + (double)P.bias[e] : s;
-    return c == -inf ? 0 : order_key(c);
+    const double b = P.bias ? (double)P.bias[e] : 0.0, c = s + b;
+    return b == -inf ? 0 : order_key(c);
   };
   wave_lds_handoff();
   for (int e = lane; e < E; e += 64) store[e] = key(e, P.groups > 1 && P.top2);
@@ -661,27 +661,32 @@ __global__ void __launch_bounds__(kThreads, resident(sizeof(T), LPR, IPL)) k_rou
       // first one left are one pair, this pair says nothing of what comes behind it: every candidate is looked at, also those
       // that the bound or the cut of equal values kept off the list.  (Larger values are in slots before, where each has been held
       // against its neighbour.)
-      const float slot_value = key_value((uint32_t)(got >> 32));
-      bool cut_same = false;
-      if (P.bias && got) {
-        const uint64_t next = slots[t + 1];
-        const float v = slot_value, v2 = key_value((uint32_t)(next >> 32));
-        if (next && v - v2 <= err + 0x1p-22f * (fabsf(v) + fabsf(v2))) {
-          const int at2 = kMaxCands - (int)(uint32_t)next;
-          const bool same = (float)src[at] == (float)src[at2] && P.bias[at] == P.bias[at2];
-          close |= !same;
-          cut_same = same && t == k - 1;
+      if (P.bias) {
+        bool cut_same = false;
+        const float v = key_value((uint32_t)(got >> 32));
+        if (got) {
+          const uint64_t next = slots[t + 1];
+          const float v2 = key_value((uint32_t)(next >> 32));
+          if (next && v - v2 <= err + 0x1p-22f * (fabsf(v) + fabsf(v2))) {
+            const int at2 = kMaxCands - (int)(uint32_t)next;
+            const bool same = (float)src[at] == (float)src[at2] && P.bias[at] == P.bias[at2];
+            close |= !same;
+            cut_same = same && t == k - 1;
+          }
         }
-      }
-      if (__any(cut_same)) {
-        const float worst = __shfl(slot_value, k - 1, LPR);
-        const int at_cut = __shfl(cut_same ? at : -1, k - 1, LPR);
-        if (at_cut >= 0 && in_group) {
-          const float l_cut = (float)src[at_cut], b_cut = P.bias[at_cut];
+        if (__any(cut_same)) {
+          const float worst = __shfl(v, k - 1, LPR);
+          const int at_cut = __shfl(cut_same ? at : -1, k - 1, LPR);
+          // from here up to `worst` fp32 cannot tell: the tolerance above with both values taken for the larger, and a little more
+          const float least = __builtin_fmaxf(worst - (err + 0x1.4p-21f * fabsf(worst)) * 1.0001f, -__FLT_MAX__);
+          uint32_t near = 0;
 #pragma unroll
-          for (int i = 0; i < IPL; ++i)
-            if (c[i] != -kInf && c[i] <= worst && worst - c[i] <= err + 0x1p-22f * (fabsf(worst) + fabsf(c[i])))
-              close |= !((float)src[first + i] == l_cut && bias[i] == b_cut);
+          for (int i = 0; i < IPL; ++i) near |= c[i] >= least && c[i] <= worst ? 1u << i : 0;
+          if (at_cut < 0 || !in_group) near = 0;
+          for (; near; near &= near - 1) {
+            const int e = first + __builtin_ctz(near);
+            close |= !((float)src[e] == (float)src[at_cut] && P.bias[e] == P.bias[at_cut]);
+          }
         }
       }
       const uint64_t all_close = __ballot(close && mine);
