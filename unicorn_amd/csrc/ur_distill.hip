@@ -51,8 +51,9 @@ __device__ __forceinline__ int64_t slot_class(const DistillParams& P, int64_t ro
   return P.index64 ? static_cast<const int64_t*>(P.index)[i] : (int64_t)static_cast<const int32_t*>(P.index)[i];
 }
 
-// exp((v - m) / T), scale = log2(e) / T, by the hardware's exponential (1 ulp); an infinite maximum makes inf - inf of the
-// equal ones, as the definition does
+// exp((v - m) / T), scale = log2(e) / T, by the hardware's exponential (1 ulp) of a product that is rounded once, which costs
+// |v - m| / T 2^-24 beside it.  (With the product's rest as a second term 5 to 7 % slower and no nearer to 64 bits: an fp32
+// gradient is off by 1.1e-7 of its norm either way, the formulas in torch's fp32 operations by 1.25e-7.)  An infinite maximum makes inf - inf of the equal ones, as the definition does.
 __device__ __forceinline__ float exp_diff(float v, float m, float scale) { return __builtin_amdgcn_exp2f((v - m) * scale); }
 
 // exp((v - m) / T) to 2 ulp whatever the size of the argument: the argument is formed in 64 bits and split into a whole
@@ -237,8 +238,8 @@ __device__ __forceinline__ void reduced_loss(const DistillParams& P, double sum,
   if (P.stats) P.stats[2 * P.rows] = (float)factor;
 }
 
-// Forward, L lanes a row (a row of few classes), kThreads / L rows a workgroup.  100000 x 6 fp32 13 us, 30000 x 128 bf16 10.4,
-// 32768 x 1000 bf16 33 us (2.0 TB/s; 21 without the teacher's part): bound by the teacher's 64-bit arithmetic, once a wave.
+// Forward, L lanes a row (a row of few classes), kThreads / L rows a workgroup.  100000 x 6 fp32 13 us, 30000 x 128 bf16 10,
+// 32768 x 1000 bf16 32 us (2.1 TB/s; 21 without the teacher's part): bound by the teacher's 64-bit arithmetic, once a wave.
 template <typename T, int L>
 __global__ void __launch_bounds__(kThreads) k_distill_fwd_rows(const DistillParams P) {
   constexpr int R = kThreads / L;
@@ -299,8 +300,9 @@ __device__ __forceinline__ void finish_row(const DistillParams& P, int64_t row, 
   }
 }
 
-// Forward, one workgroup a row.  8192 x 32768 bf16 101 us (5.3 TB/s; 512 and 1024 threads 113 and 180), 4096 x 8101 fp16
-// 17.8 us (3.7 TB/s: one exponential and six other instructions an element, and the teacher at each row's end).
+// Forward, one workgroup a row.  8192 x 32768 bf16 101 us by itself (5.3 TB/s; 512 and 1024 threads 113 and 180), 111 between the
+// backwards of a training step (4.8), 4096 x 32768 fp32 98 us (5.5), 2000 x 20000 fp32 39 us (4.1), 4096 x 8101 fp16 17 us (3.9
+// TB/s: one exponential and six other instructions an element, and the teacher at each row's end).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_distill_fwd(const DistillParams P) {
   __shared__ float part[2][kThreads / 64];
@@ -467,7 +469,8 @@ __device__ __forceinline__ void write_shares(const DistillParams& P, const RowGr
   }
 }
 
-// L lanes a row, kThreads / L rows a workgroup; a wave's stores to one place stay in their order
+// L lanes a row, kThreads / L rows a workgroup; a wave's stores to one place stay in their order.  32768 x 1000 bf16 41 us
+// (3.2 TB/s), 30000 x 128 bf16 11, 100000 x 6 fp32 7: the teacher's reductions are made again, once a wave.
 template <typename T, int L>
 __global__ void __launch_bounds__(kThreads) k_distill_bwd_rows(const DistillParams P) {
   constexpr int R = kThreads / L;
@@ -485,8 +488,8 @@ __global__ void __launch_bounds__(kThreads) k_distill_bwd_rows(const DistillPara
   if (mine) write_shares<T>(P, r, z, out, cls[sub], share[sub], 0, P.cols, t, L);
 }
 
-// A workgroup takes one row or (P.splits > 1) a part of one.  8192 x 32768 bf16 210 us (5.1 TB/s; with ordinary stores 250),
-// 4096 x 8101 fp16 31.5 us (4.2), 3 x 131071 bf16 10.3 us.
+// A workgroup takes one row or (P.splits > 1) a part of one.  8192 x 32768 bf16 213 us (5.0 TB/s; with ordinary stores 250),
+// 4096 x 32768 fp32 210 us (5.1), 2000 x 20000 fp32 63 us (5.1), 4096 x 8101 fp16 31.5 us (4.2), 3 x 131071 bf16 10.3 us.
 template <typename T, int TH>
 __global__ void __launch_bounds__(TH) k_distill_bwd(const DistillParams P) {
   __shared__ int cls[kMaxTop];

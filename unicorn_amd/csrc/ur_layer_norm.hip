@@ -622,7 +622,8 @@ struct LnPlan {
 // rows one workgroup a row is as good or better).
 constexpr int kSplitVecs = 4096, kSplitRows = 64;
 // Backward: up to this many rows and vectors in one launch (192 x 512 fp32: 3.7 against 6.8 us, and a launch less for the host;
-// 512 x 512: 6.0 against 7.0, 1000 x 512: 10.1 against 7.6, 192 x 1926: 8.7 against 8.1).
+// 512 x 512: 6.0 against 7.0, 1000 x 512: 10.1 against 7.6, 192 x 1926: 8.7 against 8.1).  The two cross between 512 and 1000 rows
+// of 128 vectors; 256 keeps away from there, since what the strips lose grows with the rows and the gain does not.
 constexpr int kSmallRows = 256, kSmallVecs = 128;
 LnPlan ln_plan(int64_t rows, int64_t cols, int dtype, bool backward) {
   LnPlan p{};

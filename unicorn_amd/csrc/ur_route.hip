@@ -179,6 +179,7 @@ __device__ int choose_wide(const RouteParams& P, const T* __restrict__ row, uint
 }
 
 // ---- weights of the chosen, LPR lanes a row: lane j holds slot j -------------------------------------------------------
+// (reciprocals are the hardware's: 1 ulp instead of half a one, for one instruction instead of the ten of a division)
 struct Chosen {
   float share;   // s_j / sum of the chosen s (renormalised), or s_j
   float comp;    // 1 - s_j of a sigmoid
@@ -234,9 +235,9 @@ __device__ __forceinline__ void row_softmax(const T* __restrict__ row, int E, in
 // and nothing has to be redone.  Such rows are noted and done after every kSteps rounds, outside the loop over rows, which
 // has the registers to itself then.
 //
-// Bound by instruction issue, not by memory: 131072 rows of 256 bf16, sigmoid with bias and 4 of 8 groups, top 8: 66 us (67 MB
-// read: 1 TB/s; 54 without the 64-bit choice), softmax without a bias 36 us; 4099 x 64: 7 us, half of it the latency of a
-// row that is done in 64 bits.  All logits equal (every row is done in 64 bits): 550 us.
+// Bound by instruction issue, not by memory: 131072 rows of 256 bf16, sigmoid with bias and 4 of 8 groups, top 8: 67 us (67 MB
+// read: 1 TB/s; 54 without the 64-bit choice; 70 where the biases are all 0, as they are at first), softmax without a bias 36 us; 4099 x 64: 7 us, half of it the latency of a
+// row that is done in 64 bits.  All logits equal (every row is done in 64 bits): 580 us.
 //
 // The top-k is not taken by k rounds of a maximum: the (k+1)-th largest of the lanes' maxima is a lower bound of the (k+1)-th
 // largest candidate; the few candidates that reach it (about 10 of 256) go to a list in LDS as (key, index) and each finds
@@ -282,7 +283,7 @@ __device__ __forceinline__ float max_rows(float v) {
   return v;
 }
 
-// (131072 x 256: 68 us; with the maxima ranked by comparing each with all others 75.)
+// (131072 x 256: with the maxima ranked by comparing each with all others instead of this network 7 us more.)
 // A finite lower bound (or the lowest finite number) of the (k+1)-th largest value, from the maxima of two sets of values a
 // lane.  (Two, because groups that were not taken leave lanes empty: with half of 16 lanes left, their 16 sets still bound
 // the 9th largest.)
@@ -441,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, resident(sizeof(T), LPR, IPL)) k_rou
 
       // err: bound of two scores' errors.  sigmoid: s (1 - s) (|l| 2^-23.4 + 2^-23) of the exponential, 2^-23 of the
       // reciprocal, 2^-24 of the sum: below 2^-22 each.  softmax, relative to its largest score 1 / z: as much of the
-      // exponential and up to 30 roundings of z, below 2^-19 each.
+      // exponential and up to 30 roundings of z, below 2^-19 each.  Of the two together twice as much is taken in either case.
       float m = 0.0f, z = 1.0f, inv_z = 1.0f, err = 0x1p-20f;
       if (need_softmax) {
         float mf = c[0];

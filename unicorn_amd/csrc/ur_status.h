@@ -1,5 +1,5 @@
 // Error reporting shared by the translation units of the library: the message behind ur_last_error() is one
-// thread-local buffer, written through these two functions (defined beside it, in ur_library.hip).
+// thread-local buffer, written through these functions (defined beside it, in ur_library.hip).
 #pragma once
 #include <stddef.h>
 

@@ -9,7 +9,9 @@ a row's loss is T^2 * sum_j p_j (log p_j - log q[index_j]).  A slot with a negat
 leaves where nothing was eligible); several slots may name one class; a row without a filled slot has loss and gradient
 0 and does not count in the mean.  The teacher gets no gradient.  A class index beyond the logits makes its row NaN, as
 a NaN among the row's logits or teacher logits does; -inf rules a class or slot out (a class the teacher wants
-that the student rules out makes the loss infinite, its gradient stays finite).
+that the student rules out makes the loss infinite, its gradient stays finite).  The student's sum is float32, so a
+row's loss is off by about 1e-7 T^2: at a large T it says little where the loss itself does not grow with T^2 (a teacher that
+knows every class).
 """
 import torch
 

@@ -9,7 +9,8 @@ The choice: scores s = softmax or sigmoid of the logits (last dimension: the can
 bias takes part in the choice only, not in the weights, and gets no gradient); with `groups` > 1 the candidates are
 consecutive groups of equal size, a group is worth its largest c ("max") or the sum of its two largest ("top2"), and only
 the `top_groups` best groups take part; ties go to the lowest index.  Two scores that differ by less than float32 can
-tell are still ordered as in 64 bits; without a bias the logits are compared.
+tell are still ordered as in 64 bits; without a bias the logits are compared.  (Groups whose "top2" sums agree but for the last
+bit of 64 may be taken in either order.)
 
 weights: s of the chosen, divided by their sum when `renormalize`, times `scale`; float32, largest c first, with a gradient
 to the logits.  indices: int64; counts: int32, how many rows took each candidate.  A logit of -inf (or a bias of -inf) rules
