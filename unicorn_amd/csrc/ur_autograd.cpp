@@ -75,12 +75,15 @@ void same_device(const Tensor& t, const Tensor& other) {
     throw std::invalid_argument("tensors must be on one device: " + t.device().str() + " and " + other.device().str());
 }
 
+// A tensor's numbers as they are in memory: a lazily negated view (`z.conj().imag`) is written out first.
+Tensor stored(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 // A tensor read as rows of its last dimension: as it lies where its rows are dense and evenly spaced without overlap (any
 // stride between them), a contiguous copy otherwise.
 struct Rows {
   Tensor t;
   int64_t rows, cols, stride;
-  explicit Rows(const Tensor& x) : t(x), cols(x.size(-1)) {
+  explicit Rows(const Tensor& x) : t(stored(x)), cols(x.size(-1)) {
     if (!t.is_contiguous()) {
       bool as_is = false;
       if (cols == 1 || t.stride(-1) == 1) {
@@ -115,7 +118,7 @@ Tensor workspace(int64_t bytes, const Tensor& like) {
 }
 void* ptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 const void* cptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
-Tensor or_none(const std::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
+Tensor or_none(const std::optional<Tensor>& t) { return t.has_value() ? stored(*t) : Tensor(); }
 
 // What the nodes know nothing of is refused.  A tangent of forward-mode differentiation would be dropped without a word.  A
 // tracer records the allocation of a result but not the kernel that fills it: the trace would return uninitialised memory.
@@ -287,7 +290,7 @@ Tensor route_backward(const Tensor& grad_weights, const Tensor& logits, const Te
                       int64_t score, bool renormalize, double scale) {
   const c10::DeviceGuard guard(logits.device());
   const Rows r(logits);
-  const Tensor g = grad_weights.contiguous();
+  const Tensor g = stored(grad_weights).contiguous();
   Tensor grad = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
   if (r.rows)
     check(api.route_backward(g.const_data_ptr<float>(), r.data(), r.stride, dtype_code(logits.scalar_type()), r.rows,
@@ -371,7 +374,7 @@ Tensor distill_backward(const Tensor& grad_loss, const Tensor& logits, const Ten
   const Rows r(logits);
   Tensor grad = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
   if (!r.rows) return grad;
-  const Tensor g = grad_loss.dim() > 1 ? grad_loss.reshape({-1}) : grad_loss;
+  const Tensor flat = stored(grad_loss), g = flat.dim() > 1 ? flat.reshape({-1}) : flat;
   check(api.distill_backward(g.const_data_ptr<float>(), g.dim() ? g.stride(0) : 0, r.data(), r.stride,
                              dtype_code(logits.scalar_type()), r.rows, r.cols, teacher.const_data_ptr(),
                              dtype_code(teacher.scalar_type()), index.const_data_ptr(), (int)index.element_size(),
@@ -407,8 +410,10 @@ struct DistillBackward : Node {
   std::string name() const override { return "DistillBackward"; }
 };
 
-Tensor distill(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature, int64_t reduction) {
-  plain_inputs({logits, teacher, index});
+Tensor distill(const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_index, double temperature,
+               int64_t reduction) {
+  plain_inputs({logits, teacher_logits, teacher_index});
+  const Tensor teacher = stored(teacher_logits), index = stored(teacher_index);
   const bool record = compute_requires_grad(logits);
   auto [loss, stats] = distill_forward(logits, teacher, index, temperature, reduction, record);
   if (record) {
