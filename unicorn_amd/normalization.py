@@ -8,7 +8,8 @@ x: float32, float16 or bfloat16, any shape and strides (rows with a dense last d
 they lie, others are copied first); weight and bias have x's type or float32.  Statistics and sums are float32, the
 result is rounded once.  The gradients of weight and bias are summed in a fixed order, at most 128 rows one after the other in
 float32 and those sums in 64 bits: the same call gives the same bits.
-No rows give an empty result and zero parameter gradients.  A row that holds an infinity or a NaN becomes NaN.
+No rows give an empty result and zero parameter gradients.  A row that holds an infinity or a NaN becomes NaN; one whose
+squares pass float32's range (numbers beyond 1e19) has no variance: NaN, or the bias.
 """
 import torch
 from torch import nn
